@@ -1,6 +1,7 @@
 // The two ends of a speculative round (gfx950): softmax rows of the LM head's logits, and the verification of drafted
 // tokens. Both are bound by the rows of the vocabulary that they read; a row is cut into segments, a workgroup each, so
-// that one row alone reaches many CUs, and a second launch joins the segments.
+// that one row alone reaches many CUs, and a second launch joins the segments. A thread takes sixteen entries of its
+// segment and requests them all before it looks at the first.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -10,20 +11,58 @@ namespace spec {
 namespace {
 
 constexpr int kInvalid = 1;                       // hipErrorInvalidValue
-constexpr int THREADS = 256;
-constexpr int SEG = 4096;                         // entries of a row per workgroup
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int OWN = 16;                           // entries per thread
+constexpr int SEG = THREADS * OWN;                // entries of a row per workgroup
 
 typedef long long ll;
 
-__device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
-__device__ __forceinline__ float get(const float* p, ll i) { return p[i]; }
-__device__ __forceinline__ float get(const uint16_t* p, ll i) { return widen(p[i]); }
+// Vectors at any address that their elements may have: global memory takes 128 bits from there.
+typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+
+// N consecutive entries of a row as f32, `fill` from entry `left` on.
+template <int N>
+__device__ __forceinline__ void load(const float* p, int left, float fill, float (&x)[N]) {
+    if (left >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i < left ? p[i] : fill;
+    }
+}
+template <int N>
+__device__ __forceinline__ void load(const uint16_t* p, int left, float fill, float (&x)[N]) {
+    if (left >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(p + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[i + 2 * e] = __uint_as_float(v[e] << 16);
+                x[i + 2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i < left ? __uint_as_float((uint32_t)p[i] << 16) : fill;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- probabilities
 
 // A segment's greatest logit and where it first stands, and the sum of exp((x - greatest) / T) over it.
 struct Part {
     float top, sum;
     int at, pad;
 };
+
+constexpr float kNone = -__builtin_inff();
 
 __device__ __forceinline__ bool before(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
@@ -34,37 +73,59 @@ __device__ __forceinline__ float rate_of(const float* temperature, int r) {
 }
 
 // exp((x - top) * rate), 0 for -inf (also where nothing else is there and top is -inf).
-__device__ __forceinline__ float share(float x, float top, float rate) {
-    return x == -__builtin_inff() ? 0.0f : expf((x - top) * rate);
-}
+__device__ __forceinline__ float share(float x, float top, float rate) { return x == kNone ? 0.0f : expf((x - top) * rate); }
 
-template <typename L>
-__global__ void __launch_bounds__(THREADS) probs_parts_kernel(int vocab, const L* logits, ll ldl, const float* temperature,
-                                                              Part* parts) {
-    const int r = blockIdx.y, seg = blockIdx.x, t = threadIdx.x;
-    const L* row = logits + r * ldl;
-    const int lo = seg * SEG, hi = min(vocab - lo, SEG) + lo;
-    const float rate = rate_of(temperature, r);
-    float top = -__builtin_inff();
-    int at = 0x7fffffff;
-    for (int i = lo + t; i < hi; i += THREADS) {
-        const float x = get(row, i);
-        if (before(x, i, top, at)) top = x, at = i;
-    }
-    __shared__ float tops[4], sums[4];
-    __shared__ int ats[4];
+__device__ __forceinline__ void wave_top(float& top, int& at) {
+#pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
         const float x = __shfl_xor(top, m, 64);
         const int i = __shfl_xor(at, m, 64);
         if (before(x, i, top, at)) top = x, at = i;
     }
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
+    return x;
+}
+
+// Groups of four (f32) or eight (bf16) entries go around the threads, so that a wave's access is contiguous.
+template <typename L> constexpr int kGroup = 16 / sizeof(L);
+
+template <typename L>
+__global__ void __launch_bounds__(THREADS) probs_parts_kernel(int vocab, const L* logits, ll ldl, const float* temperature,
+                                                              Part* parts) {
+    constexpr int G = kGroup<L>;
+    const int r = blockIdx.y, seg = blockIdx.x, t = threadIdx.x;
+    const L* row = logits + r * ldl;
+    float x[OWN / G][G];
+#pragma unroll
+    for (int j = 0; j < OWN / G; ++j) {
+        const int i = seg * SEG + (j * THREADS + t) * G;
+        load<G>(row + i, vocab - i, kNone, x[j]);
+    }
+    const float rate = rate_of(temperature, r);
+    float top = kNone;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < OWN / G; ++j)
+#pragma unroll
+        for (int e = 0; e < G; ++e)
+            if (x[j][e] > top) top = x[j][e], at = seg * SEG + (j * THREADS + t) * G + e;
+    __shared__ float tops[WAVES], sums[WAVES];
+    __shared__ int ats[WAVES];
+    wave_top(top, at);
     if ((t & 63) == 0) tops[t >> 6] = top, ats[t >> 6] = at;
     __syncthreads();
-    for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
         if (before(tops[w], ats[w], top, at)) top = tops[w], at = ats[w];
     float sum = 0.0f;
-    for (int i = lo + t; i < hi; i += THREADS) sum += share(get(row, i), top, rate);
-    for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m, 64);
+#pragma unroll
+    for (int j = 0; j < OWN / G; ++j)
+#pragma unroll
+        for (int e = 0; e < G; ++e) sum += share(x[j][e], top, rate);
+    sum = wave_sum(sum);
     if ((t & 63) == 0) sums[t >> 6] = sum;
     __syncthreads();
     if (t == 0) parts[(ll)r * gridDim.x + seg] = {top, (sums[0] + sums[1]) + (sums[2] + sums[3]), at, 0};
@@ -73,27 +134,49 @@ __global__ void __launch_bounds__(THREADS) probs_parts_kernel(int vocab, const L
 template <typename L>
 __global__ void __launch_bounds__(THREADS) probs_write_kernel(int vocab, const L* logits, ll ldl, const float* temperature,
                                                               float* probs, ll ldp, const Part* parts) {
-    const int r = blockIdx.y, seg = blockIdx.x, segs = gridDim.x, t = threadIdx.x;
-    const Part* p = parts + (ll)r * segs;
-    float top = -__builtin_inff();
-    int at = 0x7fffffff;
-    for (int i = 0; i < segs; ++i)
-        if (before(p[i].top, p[i].at, top, at)) top = p[i].top, at = p[i].at;
-    const float rate = rate_of(temperature, r);
-    const int lo = seg * SEG, hi = min(vocab - lo, SEG) + lo;
-    float* dst = probs + r * ldp;
-    if (rate == 0.0f) {
-        for (int i = lo + t; i < hi; i += THREADS) dst[i] = i == at && top > -__builtin_inff() ? 1.0f : 0.0f;
-        return;
-    }
-    float sum = 0.0f;
-    for (int i = 0; i < segs; ++i) sum += share(p[i].top, top, rate) * p[i].sum;
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    constexpr int G = kGroup<L>;
+    const int r = blockIdx.y, seg = blockIdx.x, segs = gridDim.x, t = threadIdx.x, lane = t & 63;
     const L* row = logits + r * ldl;
-    for (int i = lo + t; i < hi; i += THREADS) dst[i] = share(get(row, i), top, rate) * by;
+    float x[OWN / G][G];
+#pragma unroll
+    for (int j = 0; j < OWN / G; ++j) {
+        const int i = seg * SEG + (j * THREADS + t) * G;
+        load<G>(row + i, vocab - i, kNone, x[j]);
+    }
+    const float rate = rate_of(temperature, r);
+    const Part* p = parts + (ll)r * segs;
+    float top = kNone;
+    int at = 0x7fffffff;
+    for (int i = lane; i < segs; i += 64)         // every wave for itself
+        if (before(p[i].top, p[i].at, top, at)) top = p[i].top, at = p[i].at;
+    wave_top(top, at);
+    float* dst = probs + r * ldp;
+    float by = 0.0f;
+    if (rate != 0.0f) {
+        float sum = 0.0f;
+        for (int i = lane; i < segs; i += 64) sum += share(p[i].top, top, rate) * p[i].sum;
+        sum = wave_sum(sum);
+        by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    }
+#pragma unroll
+    for (int j = 0; j < OWN / G; ++j) {
+        const int i = seg * SEG + (j * THREADS + t) * G;
+        float y[G];
+#pragma unroll
+        for (int e = 0; e < G; ++e)
+            y[e] = rate != 0.0f ? share(x[j][e], top, rate) * by : i + e == at && top > kNone ? 1.0f : 0.0f;
+        if (vocab - i >= G) {
+#pragma unroll
+            for (int e = 0; e < G; e += 4) *reinterpret_cast<f32x4*>(dst + i + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+                if (i + e < vocab) dst[i + e] = y[e];
+        }
+    }
 }
 
-// ---------------------------------------------------------------------------------------------------------------
+// ---------------------------------------------------------------------------------------------------- verification
 
 __device__ __forceinline__ double weight(float p) { return p > 0.0f && p < __builtin_inff() ? (double)p : 0.0; }
 
@@ -108,18 +191,15 @@ struct Accept {
     const float* uniform;
 };
 
-// Request b's outcome: `kept` rows, the last of them global row `last`, and whether row last + 1 was rejected. Every
-// thread of the workgroup computes it (a wave at a time looks at 64 drafted rows).
+// Request b's outcome: `kept` rows, and whether the row behind them was rejected. Every wave computes it, 64 drafted rows
+// at a time.
 struct Outcome {
-    ll last;
     int kept;
     bool rejected;
 };
 
-__device__ __forceinline__ Outcome outcome(const Accept& a, int b) {
-    const ll first = a.cu_rows[b];
-    const int n = a.cu_rows[b + 1] - (int)first;
-    if (n <= 0) return {first, 0, false};
+__device__ __forceinline__ Outcome outcome(const Accept& a, ll first, int n) {
+    if (n <= 0) return {0, false};
     const int lane = threadIdx.x & 63;
     for (int i0 = 1; i0 < n; i0 += 64) {
         const int i = i0 + lane;
@@ -132,12 +212,9 @@ __device__ __forceinline__ Outcome outcome(const Accept& a, int b) {
                       weight(a.target[(r - 1) * a.p_stride + x]);
         }
         const unsigned long long no = __ballot(!yes);
-        if (no) {
-            const int kept = i0 + __builtin_ctzll(no);
-            return {first + kept - 1, kept, true};
-        }
+        if (no) return {i0 + __builtin_ctzll(no), true};
     }
-    return {first + n - 1, n, false};
+    return {n, false};
 }
 
 // What the next token is drawn from: p of the last kept row, less q where a draft was rejected behind it.
@@ -145,104 +222,177 @@ struct Weights {
     const float* p;
     const float* q;                               // NULL: none
     int without;                                  // a certain draft's token, -1: none
-    __device__ __forceinline__ double at(int i) const {
-        double w = weight(p[i]);
-        if (q) w = fmax(w - weight(q[i]), 0.0);
-        return i == without ? 0.0 : w;
+
+    // The weights of N entries from i on, 0 behind the vocabulary.
+    template <int N>
+    __device__ __forceinline__ void get(int i, int vocab, double (&w)[N]) const {
+        float x[N], y[N];
+        load<N>(p + i, vocab - i, 0.0f, x);
+        if (q) load<N>(q + i, vocab - i, 0.0f, y);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            w[e] = weight(x[e]);
+            if (q) w[e] = fmax(w[e] - weight(y[e]), 0.0);
+            if (i + e == without) w[e] = 0.0;
+        }
     }
 };
 
-__device__ __forceinline__ Weights weights(const Accept& a, const Outcome& o) {
-    Weights w{a.target + o.last * a.p_stride, nullptr, -1};
+__device__ __forceinline__ Weights weights(const Accept& a, ll first, Outcome o) {
+    const ll last = first + o.kept - 1;
+    Weights w{a.target + last * a.p_stride, nullptr, -1};
     if (o.rejected) {
-        if (a.draft) w.q = a.draft + (o.last + 1) * a.q_stride;
-        else w.without = a.tokens[o.last + 1];
+        if (a.draft) w.q = a.draft + (last + 1) * a.q_stride;
+        else w.without = a.tokens[last + 1];
     }
     return w;
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
     for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
     return x;
 }
 
-__global__ void __launch_bounds__(THREADS) accept_parts_kernel(const Accept a, double* parts) {
+// Each segment's sum of weights, and with the first segment the request's outcome.
+__global__ void __launch_bounds__(THREADS) accept_parts_kernel(const Accept a, double* parts, int32_t* outcomes) {
     const int b = blockIdx.y, seg = blockIdx.x, t = threadIdx.x;
-    const Outcome o = outcome(a, b);
-    __shared__ double sums[4];
+    const ll first = a.cu_rows[b];
+    const Outcome o = outcome(a, first, a.cu_rows[b + 1] - (int)first);
+    __shared__ double sums[WAVES];
     double sum = 0.0;
     if (o.kept > 0) {
-        const Weights w = weights(a, o);
-        const int lo = seg * SEG, hi = min(a.vocab - lo, SEG) + lo;
-        for (int i = lo + t; i < hi; i += THREADS) sum += w.at(i);
+        const Weights w = weights(a, first, o);
+        double x[OWN / 4][4];
+#pragma unroll
+        for (int j = 0; j < OWN / 4; ++j) w.get<4>(seg * SEG + (j * THREADS + t) * 4, a.vocab, x[j]);
+#pragma unroll
+        for (int j = 0; j < OWN / 4; ++j) sum += (x[j][0] + x[j][1]) + (x[j][2] + x[j][3]);
     }
     sum = wave_sum(sum);
     if ((t & 63) == 0) sums[t >> 6] = sum;
     __syncthreads();
-    if (t == 0) parts[(ll)b * gridDim.x + seg] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    if (t == 0) {
+        parts[(ll)b * gridDim.x + seg] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        if (seg == 0) outcomes[b] = o.rejected ? -o.kept : o.kept;
+    }
 }
 
-// The lowest entry of [lo, hi) whose weight brings `sum` over `edge`, or the last entry with a weight where rounding
-// leaves none. Each thread takes a run of consecutive entries; the threads' sums meet in LDS.
-__device__ int crossing(const Weights& w, int lo, int hi, double sum, double edge, double* sums, int* found) {
-    const int t = threadIdx.x, run = (hi - lo + THREADS - 1) / THREADS;
-    const int mine = min(lo + t * run, hi), end = min(mine + run, hi);
-    double own = 0.0;
-    int some = -1;
-    for (int i = mine; i < end; ++i) {
-        const double x = w.at(i);
-        own += x;
-        if (x > 0.0) some = i;
-    }
-    sums[t] = own;
-    if (t == 0) found[0] = 0x7fffffff, found[1] = -1;
-    __syncthreads();
-    for (int i = 0; i < t; ++i) sum += sums[i];
-    if (some >= 0) atomicMax(&found[1], some);
-    for (int i = mine; i < end; ++i) {
-        sum += w.at(i);
-        if (sum > edge) {
-            atomicMin(&found[0], i);
-            break;
-        }
+struct Scratch {
+    double sums[WAVES];
+    int over[WAVES], some[WAVES];
+};
+
+// The sum over the threads before this one, and over all of them. Every thread calls it.
+__device__ __forceinline__ double scan(double own, double& all, Scratch& s) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    double x = own;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double y = __shfl_up(x, m, 64);
+        if (lane >= m) x += y;
     }
     __syncthreads();
-    return found[0] != 0x7fffffff ? found[0] : found[1];
+    if (lane == 63) s.sums[wave] = x;
+    __syncthreads();
+    all = 0.0;
+    double ahead = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) ahead += s.sums[w];
+        all += s.sums[w];
+    }
+    const double y = __shfl_up(x, 1, 64);
+    return ahead + (lane > 0 ? y : 0.0);
 }
 
-__global__ void __launch_bounds__(THREADS) accept_pick_kernel(const Accept a, int segs, const double* parts, int32_t* keep,
-                                                              int32_t* next) {
+// The least `over` of all threads (0x7fffffff: none), or where there is none the greatest `some` (-1: none).
+__device__ __forceinline__ int pick(int over, int some, Scratch& s) {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        over = min(over, __shfl_xor(over, m, 64));
+        some = max(some, __shfl_xor(some, m, 64));
+    }
+    __syncthreads();
+    if ((t & 63) == 0) s.over[t >> 6] = over, s.some[t >> 6] = some;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) over = min(over, s.over[w]), some = max(some, s.some[w]);
+    return over != 0x7fffffff ? over : some;
+}
+
+// The lowest entry of the segment from `lo` on whose weight brings `sum` over `edge`; where rounding leaves none, the last
+// one with a weight. `sum` gets the segment's added.
+__device__ __forceinline__ int crossing(const Weights& w, int lo, int vocab, double& sum, double edge, Scratch& s, bool& over_edge) {
+    const int mine = lo + threadIdx.x * OWN;
+    double x[OWN], own = 0.0, all;
+    w.get<OWN>(mine, vocab, x);
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) own += x[e];
+    double run = sum + scan(own, all, s);
+    int over = 0x7fffffff, some = -1;
+#pragma unroll
+    for (int e = 0; e < OWN; ++e) {
+        run += x[e];
+        if (x[e] > 0.0) some = mine + e;
+        if (run > edge && over == 0x7fffffff && x[e] > 0.0) over = mine + e;
+    }
+    const int best = pick(over, some, s);
+    sum += all;
+    over_edge = sum > edge;
+    return best;
+}
+
+__global__ void __launch_bounds__(THREADS) accept_pick_kernel(const Accept a, int segs, const double* parts,
+                                                              const int32_t* outcomes, int32_t* keep, int32_t* next) {
     const int b = blockIdx.x, t = threadIdx.x;
-    const Outcome o = outcome(a, b);
-    __shared__ double sums[THREADS];
-    __shared__ int found[2];
+    __shared__ Scratch s;
+    const int code = outcomes[b];
+    const Outcome o{code < 0 ? -code : code, code < 0};
+    const ll first = a.cu_rows[b];
     int token = -1;
     if (o.kept > 0) {
-        Weights w = weights(a, o);
+        Weights w = weights(a, first, o);
         const double* p = parts + (ll)b * segs;
-        const double u = a.uniform[a.cu_rows[b]];
-        double all = 0.0;
-        for (int i = 0; i < segs; ++i) all += p[i];
+        const double u = a.uniform[first];
+        // a run of consecutive segments per thread
+        const int run = (segs + THREADS - 1) / THREADS, lo = min(t * run, segs), hi = min(lo + run, segs);
+        double own = 0.0, all;
+        for (int i = lo; i < hi; ++i) own += p[i];
+        const double ahead = scan(own, all, s);
+        bool done;
         if (all > 0.0) {
             const double edge = u * all;
-            double sum = 0.0, start = 0.0;
-            int seg = -1;
-            for (int i = 0; i < segs; ++i) {
-                if (p[i] > 0.0) seg = i, start = sum;
+            double sum = ahead;
+            int over = 0x7fffffff, some = -1;
+            for (int i = lo; i < hi; ++i) {
                 sum += p[i];
-                if (sum > edge) break;
+                if (p[i] > 0.0) some = i;
+                if (sum > edge && over == 0x7fffffff && p[i] > 0.0) over = i;
             }
-            token = crossing(w, seg * SEG, min(a.vocab - seg * SEG, SEG) + seg * SEG, start, edge, sums, found);
+            const int seg = pick(over, some, s);
+            // the sum ahead of that segment, from the thread that has it
+            __shared__ double start;
+            if (seg >= lo && seg < hi) {
+                double x = ahead;
+                for (int i = lo; i < seg; ++i) x += p[i];
+                start = x;
+            }
+            __syncthreads();
+            double from = start;
+            token = crossing(w, seg * SEG, a.vocab, from, edge, s, done);
         } else if (o.rejected) {
-            // the draft covers the target everywhere: p itself
+            // the draft covers the target everywhere: p itself, all of it here
             w.q = nullptr, w.without = -1;
-            double own = 0.0;
-            for (int i = t; i < a.vocab; i += THREADS) own += w.at(i);
-            sums[t] = own;
-            __syncthreads();
-            for (int i = 0; i < THREADS; ++i) all += sums[i];
-            __syncthreads();
-            if (all > 0.0) token = crossing(w, 0, a.vocab, 0.0, u * all, sums, found);
+            double whole = 0.0, sum = 0.0;
+            for (int seg = 0; seg < segs; ++seg) (void)crossing(w, seg * SEG, a.vocab, whole, 0.0, s, done);
+            const double edge = u * whole;
+            done = false;
+            for (int seg = 0; seg < segs && !done; ++seg) {
+                const int x = crossing(w, seg * SEG, a.vocab, sum, edge, s, done);
+                if (x >= 0) token = x;
+            }
         }
     }
     if (t == 0) keep[b] = o.kept, next[b] = token;
@@ -251,11 +401,21 @@ __global__ void __launch_bounds__(THREADS) accept_pick_kernel(const Accept a, in
 inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline ll segments(int vocab) { return ((ll)vocab + SEG - 1) / SEG; }
 
+template <typename L>
+int32_t probs(int rows, int vocab, const void* logits, ll ldl, const float* temperature, float* out, ll ldp, Part* parts,
+              hipStream_t stream) {
+    const dim3 grid((unsigned)segments(vocab), (unsigned)rows);
+    const L* x = static_cast<const L*>(logits);
+    probs_parts_kernel<L><<<grid, THREADS, 0, stream>>>(vocab, x, ldl, temperature, parts);
+    probs_write_kernel<L><<<grid, THREADS, 0, stream>>>(vocab, x, ldl, temperature, out, ldp, parts);
+    return (int32_t)hipGetLastError();
+}
+
 }  // namespace
 }  // namespace spec
 
 extern "C" int64_t glm53f_spec_probs_workspace_bytes(int32_t rows, int32_t vocab) {
-    if (rows < 0 || vocab < 1) return -1;
+    if (rows < 0 || rows > 65535 || vocab < 1) return -1;
     return rows * spec::segments(vocab) * (int64_t)sizeof(spec::Part);
 }
 
@@ -270,20 +430,13 @@ extern "C" int32_t glm53f_spec_probs(int32_t rows, int32_t vocab, const void* lo
         return kInvalid;
     if (logits == probs && (!logits_f32 || ldl != ldp)) return kInvalid;
     Part* parts = static_cast<Part*>(workspace);
-    const dim3 grid((unsigned)segments(vocab), (unsigned)rows);
-    if (logits_f32) {
-        probs_parts_kernel<float><<<grid, THREADS, 0, stream>>>(vocab, static_cast<const float*>(logits), ldl, temperature, parts);
-        probs_write_kernel<float><<<grid, THREADS, 0, stream>>>(vocab, static_cast<const float*>(logits), ldl, temperature, probs, ldp, parts);
-    } else {
-        probs_parts_kernel<uint16_t><<<grid, THREADS, 0, stream>>>(vocab, static_cast<const uint16_t*>(logits), ldl, temperature, parts);
-        probs_write_kernel<uint16_t><<<grid, THREADS, 0, stream>>>(vocab, static_cast<const uint16_t*>(logits), ldl, temperature, probs, ldp, parts);
-    }
-    return (int32_t)hipGetLastError();
+    return logits_f32 ? spec::probs<float>(rows, vocab, logits, ldl, temperature, probs, ldp, parts, stream)
+                      : spec::probs<uint16_t>(rows, vocab, logits, ldl, temperature, probs, ldp, parts, stream);
 }
 
 extern "C" int64_t glm53f_spec_accept_workspace_bytes(int32_t batch, int32_t vocab) {
-    if (batch < 0 || vocab < 1) return -1;
-    return batch * spec::segments(vocab) * (int64_t)sizeof(double);
+    if (batch < 0 || batch > 65535 || vocab < 1) return -1;
+    return batch * (spec::segments(vocab) * (int64_t)sizeof(double) + (int64_t)sizeof(int32_t));
 }
 
 extern "C" int32_t glm53f_spec_accept(int32_t batch, int32_t vocab, const int32_t* cu_rows, const int32_t* tokens,
@@ -297,10 +450,11 @@ extern "C" int32_t glm53f_spec_accept(int32_t batch, int32_t vocab, const int32_
         !aligned(tokens, 4) || !aligned(target, 4) || !aligned(draft, 4) || !aligned(uniform, 4) || !aligned(keep, 4) ||
         !aligned(next, 4) || !aligned(workspace, 16) || workspace_bytes < glm53f_spec_accept_workspace_bytes(batch, vocab))
         return kInvalid;
-    double* parts = static_cast<double*>(workspace);
-    const Accept a{vocab, cu_rows, tokens, target, p_stride, draft, q_stride, uniform};
     const int segs = (int)segments(vocab);
-    accept_parts_kernel<<<dim3((unsigned)segs, (unsigned)batch), THREADS, 0, stream>>>(a, parts);
-    accept_pick_kernel<<<dim3((unsigned)batch), THREADS, 0, stream>>>(a, segs, parts, keep, next);
+    double* parts = static_cast<double*>(workspace);
+    int32_t* outcomes = reinterpret_cast<int32_t*>(parts + (ll)batch * segs);
+    const Accept a{vocab, cu_rows, tokens, target, p_stride, draft, q_stride, uniform};
+    accept_parts_kernel<<<dim3((unsigned)segs, (unsigned)batch), THREADS, 0, stream>>>(a, parts, outcomes);
+    accept_pick_kernel<<<dim3((unsigned)batch), THREADS, 0, stream>>>(a, segs, parts, outcomes, keep, next);
     return (int32_t)hipGetLastError();
 }
