@@ -1,85 +1,370 @@
-// BF16 matrix product with bias, activation and residual in its epilogue (gfx950).
+// BF16 matrix product with bias, activation and residual in its epilogue (gfx950), for any rows, n and k.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "ext/glm53f_fwd_gemm.h"
 #include "fwd_epilogue.h"
+#include "fwd_stream.h"
 
 namespace fwd_fused {
 namespace {
 
 using fwd_epilogue::Epilogue;
+using fwd_stream::bf16x8;
+using fwd_stream::dropped;
+using fwd_stream::f32x4;
+using fwd_stream::u32x4;
+using fwd_stream::u32x4_any;
 
 constexpr int kInvalid = 1;                       // hipErrorInvalidValue
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr int kCus = 256;
 
 struct Args {
     const uint16_t* x;
     long long ldx, x_gs;
     const uint16_t* w;
     long long ldw, w_gs;
-    int rows, n, k;
+    int groups, rows, n, k;
     Epilogue e;
+    hipStream_t stream;
 };
 
-// Any size, any stride: a workgroup of four waves owns 64 rows x 64 outputs, both operands pass through LDS in steps of
-// 32 along k, zero beyond the edges. VEC: rows are read in pieces of 16 bytes.
-template <bool VEC>
-__global__ void __launch_bounds__(256) any_kernel(const Args a) {
-    constexpr int BM = 64, BN = 64, BK = 32, LD = BK + 8;
-    __shared__ __align__(16) uint16_t xs[BM * LD], ws[BN * LD];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, g = blockIdx.z;
-    const long long m0 = (long long)blockIdx.y * BM;
-    const int n0 = blockIdx.x * BN, tr = t >> 2, tc = (t & 3) * 8;
-    const bool xin = m0 + tr < a.rows, win = n0 + tr < a.n;
-    const uint16_t* x = a.x + g * a.x_gs + (xin ? m0 + tr : 0) * a.ldx;
-    const uint16_t* w = a.w + g * a.w_gs + (long long)(win ? n0 + tr : 0) * a.ldw;
-    auto piece = [&](const uint16_t* src, bool in, int k0) {
-        u32x4 p = {0, 0, 0, 0};
-        if (in) {
-            if constexpr (VEC) {
-                if (k0 < a.k) p = *reinterpret_cast<const u32x4*>(src + k0);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (k0 + i < a.k) p[i / 2] |= (uint32_t)src[k0 + i] << (16 * (i & 1));
-            }
-        }
-        return p;
-    };
-    f32x4 acc[2][2] = {};
-    const int mw = (wave & 1) * 32, nw = (wave >> 1) * 32;
-    for (int k0 = 0; k0 < a.k; k0 += BK) {
-        const u32x4 px = piece(x, xin, k0 + tc), pw = piece(w, win, k0 + tc);
-        __syncthreads();
-        *reinterpret_cast<u32x4*>(&xs[tr * LD + tc]) = px;
-        *reinterpret_cast<u32x4*>(&ws[tr * LD + tc]) = pw;
-        __syncthreads();
-        bf16x8 fx[2], fw[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fx[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&xs[(mw + 16 * i + (lane & 15)) * LD + 8 * (lane >> 4)]));
-            fw[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(&ws[(nw + 16 * i + (lane & 15)) * LD + 8 * (lane >> 4)]));
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[j], fx[i], acc[i][j], 0, 0, 0);
+// What the streaming kernel's four outputs become.
+struct Finish {
+    Epilogue e;
+    int n;
+    __device__ __forceinline__ void operator()(int g, int row, int o, f32x4 s) const {
+        fwd_epilogue::finish(e, fwd_epilogue::request(e, g, row, o, n), g, row, o, n, s);
     }
-    // acc[i][j][c]: row 16 i + lane % 16, output 16 j + 4 (lane / 16) + c of the wave's tile
+};
+
+// ------------------------------------------------------------------------------------------------------- tiles
+
+// 16 bytes per lane from global memory to LDS without a register in between: to lds + 16 lane (lds the same in all lanes).
+// Written out because the compiler cannot tell the two sets of tiles apart and has every read of one wait for the
+// loads of the other; whoever reads the set waits for its loads himself, before a barrier.
+__device__ __forceinline__ void to_lds(const uint16_t* src, uint16_t* lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)lds);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+}
+
+// BM rows x BN outputs per workgroup of WM x WN waves, k in steps of BK, a ring of STAGES sets of LDS tiles: the steps ahead
+// are requested before the current one's products, STAGES - 1 of them. A tile row is BK / 8 pieces of 16 bytes in LDS,
+// swizzled by the row so that the sixteen rows of an operand's read fall on all banks. With 16-byte aligned rows and k a
+// multiple of BK (FAST) the tiles go straight to LDS, the swizzle in the lanes' addresses; otherwise through registers, a
+// piece that crosses the row's end shifted and filled with zeros. Rows past the last repeat it and are not stored.
+template <int BM, int BN, int WM, int WN, int KW, int BK, int STAGES, bool FAST>
+__global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
+    constexpr int T = 64 * WM * WN * KW, MT = BM / WM / 16, NT = BN / WN / 16, PR = BK / 8;
+    constexpr int XP = BM * PR / T, WP = BN * PR / T, P = XP + WP;   // pieces per thread of a step
+    constexpr int AHEAD = FAST ? 1 : STAGES - 1;                     // steps that registers hold
+    static_assert(XP * T == BM * PR && WP * T == BN * PR, "whole pieces");
+    constexpr int SETS = FAST ? STAGES : 2, SET = (BM + BN) * BK;
+    constexpr int PASSES = KW * BM * BN * 4 > (128 << 10) ? 2 : 1, ROWS = BM / PASSES;   // the outputs take the tiles' place, in passes
+    constexpr int CELLS = SETS * SET > KW * ROWS * BN * 2 ? SETS * SET : KW * ROWS * BN * 2;
+    __shared__ __align__(16) uint16_t lds[CELLS];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = blockIdx.z;
+    // Consecutive workgroups go to the eight XCDs in turn: give each XCD a run of tiles, and order the tiles in bands of
+    // eight rows of tiles, column by column, so that the tiles that run at a time on an XCD are a block of both operands
+    // and its L2 serves most of what they read.
+    constexpr unsigned BAND = 8;
+    const unsigned row_tiles = (unsigned)((a.rows + (long long)BM - 1) / BM), col_tiles = (unsigned)((a.n + (long long)BN - 1) / BN);
+    const unsigned total = gridDim.x, per = total / 8, id = blockIdx.x;
+    const unsigned tile = id < per * 8 ? (id % 8) * per + id / 8 : id;
+    const unsigned band = tile / (BAND * col_tiles), in_band = tile % (BAND * col_tiles), high = min(BAND, row_tiles - band * BAND);
+    const long long m0 = (long long)(band * BAND + in_band % high) * BM;
+    const int n0 = (int)(in_band / high) * BN;
+    const uint16_t* x = a.x + g * a.x_gs;
+    const uint16_t* w = a.w + g * a.w_gs;
+
+    // piece i of this thread: LDS slot i T + t, row slot / PR, piece (slot mod PR) ^ swizzle of the step
+    auto swizzle = [](int row) { return PR >= 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
+    const uint16_t* src[P];
+    int col[P];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < P; ++i) {
+        const int slot = (i < XP ? i : i - XP) * T + t, row = slot / PR;
+        col[i] = 8 * ((slot & (PR - 1)) ^ swizzle(row));
+        src[i] = i < XP ? x + min(m0 + row, (long long)a.rows - 1) * a.ldx : w + (long long)min(n0 + row, a.n - 1) * a.ldw;
+    }
+    const int steps = (a.k + BK - 1) / BK;
+    u32x4 held[AHEAD][FAST ? 1 : P];
+    auto slot_of = [&](int i, int set) { return lds + set * SET + (i < XP ? i * T * 8 : BM * BK + (i - XP) * T * 8); };
+    auto request_piece = [&](int i, int step, int set) {   // (behind the last step it is requested again: the waits count requests)
+        step = min(step, steps - 1);
+        if constexpr (FAST)
+            to_lds(src[i] + step * BK + col[i], slot_of(i, set) + wave * 512);
+        else
+            held[set][i] = *reinterpret_cast<const u32x4_any*>(src[i] + min(step * BK + col[i], a.k - 8));
+    };
+    auto request = [&](int step, int set) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < P; ++i) request_piece(i, step, set);
+    };
+    auto place = [&](int step, int from, int set) {   // the registers' pieces
+        if constexpr (!FAST) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const long long m = m0 + mw + 16 * i + (lane & 15);
-                const int o = n0 + nw + 16 * j + 4 * (lane >> 4) + c;
-                if (m < a.rows && o < a.n) fwd_epilogue::finish(a.e, g, m, o, acc[i][j][c]);
+            for (int i = 0; i < P; ++i) {
+                if (step >= steps - 1) held[from][i] = dropped(held[from][i], max((steps - 1) * BK + col[i] - (a.k - 8), 0));
+                *reinterpret_cast<u32x4*>(slot_of(i, set) + t * 8) = held[from][i];
             }
+        }
+    };
+    f32x4 acc[MT][NT] = {};
+    const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) % WN * (BN / WN), wk = wave / (WM * WN), r16 = lane & 15, q = lane >> 4;
+
+    // One step's products; `between` is called P times, spread over them.
+    auto products = [&](int set, auto between) {
+        const uint16_t* xs = lds + set * SET + (wm + r16) * BK;
+        const uint16_t* ws = lds + set * SET + BM * BK + (wn + r16) * BK;
+        constexpr int KK = BK / 32 / KW, GROUPS = KK * MT;
+        bf16x8 fx[KK][MT], fw[KK][NT];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            const int at = 8 * ((4 * (wk * KK + kk) + q) ^ swizzle(r16));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fw[kk][j] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(ws + 16 * j * BK + at));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fx[kk][i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(xs + 16 * i * BK + at));
+        }
+        if constexpr (FAST) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[kk][j], fx[kk][i], acc[i][j], 0, 0, 0);
+                if constexpr (FAST) {
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int m = (kk * MT + i) * P / GROUPS; m < (kk * MT + i + 1) * P / GROUPS; ++m) between(m);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+    };
+    if constexpr (FAST && BK == 32) {
+        // The operands of the next step are read while the current one's products run.
+        bf16x8 f[2][MT + NT];
+        auto read = [&](int set, bf16x8 (&to)[MT + NT]) {
+            const uint16_t* xs = lds + set * SET + (wm + r16) * BK + 8 * (q ^ swizzle(r16));
+            const uint16_t* ws = lds + set * SET + BM * BK + (wn + r16) * BK + 8 * (q ^ swizzle(r16));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) to[i] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(xs + 16 * i * BK));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) to[MT + j] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(ws + 16 * j * BK));
+        };
+        auto multiply = [&](const bf16x8 (&by)[MT + NT]) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(by[MT + j], by[i], acc[i][j], 0, 0, 0);
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) request(s, s);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(P * (STAGES - 2)) : "memory");
+        __syncthreads();
+        read(0, f[0]);
+        int set = 0;
+        auto step = [&](int s, const bf16x8 (&now)[MT + NT], bf16x8 (&then)[MT + NT]) {
+            // step s + 1 is there behind this barrier, and everybody has the operands of s - 1 in use: its set is filled anew
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(P * (STAGES - 3)) : "memory");
+            __syncthreads();
+            const int before = set == 0 ? STAGES - 1 : set - 1;
+            set = set == STAGES - 1 ? 0 : set + 1;
+            read(set, then);
+            request(s + STAGES - 1, before);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            multiply(now);
+            __builtin_amdgcn_s_setprio(0);
+        };
+        int s = 0;
+        for (; s + 1 < steps; s += 2) {
+            step(s, f[0], f[1]);
+            step(s + 1, f[1], f[0]);
+        }
+        if (s < steps) step(s, f[0], f[1]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else if constexpr (FAST) {
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) request(s, s);
+        int set = 0;
+        for (int s = 0; s < steps; ++s) {
+            // this wave's part of the set is there once all but the newer steps' requests have come back; behind the
+            // barrier everybody's is, and nobody reads the set before it any more, which the newest request fills
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(P * (STAGES - 2)) : "memory");
+            __syncthreads();
+            products(set, [&](int i) { request_piece(i, s + STAGES - 1, set == 0 ? STAGES - 1 : set - 1); });
+            set = set == STAGES - 1 ? 0 : set + 1;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) request(s, s);
+        place(0, 0, 0);
+        request(AHEAD, 0);
+        // LDS set s mod 2 holds step s; registers s + 1 .. s + AHEAD, step i in held[i mod AHEAD]
+        for (int s0 = 0; s0 < steps; s0 += 2 * AHEAD) {
+#pragma unroll
+            for (int i = 0; i < 2 * AHEAD; ++i) {
+                const int s = s0 + i;
+                if (s >= steps) break;
+                __syncthreads();
+                products(i & 1, [](int) {});
+                place(s + 1, (i + 1) % AHEAD, (i + 1) & 1);
+                request(s + 1 + AHEAD, (i + 1) % AHEAD);
+            }
+        }
+    }
+    // acc[i][j][e]: row 16 i + lane % 16, output 16 j + 4 (lane / 16) + e of the wave's part. Through LDS (pieces of four
+    // outputs, swizzled like the tiles), so that a wave stores whole runs of a row and the epilogue is written once.
+    float* whole = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+        __syncthreads();
+        if (PASSES == 1 || wm / ROWS == pass) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int row = wm - pass * ROWS + 16 * i + r16, piece = (wn + 16 * j) / 4 + q;
+                    *reinterpret_cast<f32x4*>(&whole[wk * (ROWS * BN) + row * BN + 4 * (piece ^ (row & 7))]) = acc[i][j];
+                }
+        }
+        __syncthreads();
+        // several pieces at a time: their bias and residual are requested together
+        constexpr int U = ROWS * BN / 4 / T < 4 ? ROWS * BN / 4 / T : 4;
+        static_assert(ROWS * BN / 4 % (U * T) == 0, "whole rounds");
+        for (int s0 = t; s0 < ROWS * BN / 4; s0 += U * T) {
+            fwd_epilogue::Added added[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long m = m0 + pass * ROWS + (s0 + u * T) / (BN / 4);
+                const int o = n0 + 4 * ((s0 + u * T) % (BN / 4));
+                if (m < a.rows && o < a.n) added[u] = fwd_epilogue::request(a.e, g, m, o, a.n);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int row = (s0 + u * T) / (BN / 4), piece = (s0 + u * T) % (BN / 4);
+                const long long m = m0 + pass * ROWS + row;
+                const int o = n0 + 4 * piece;
+                if (m >= a.rows || o >= a.n) continue;
+                const float* at = &whole[row * BN + 4 * (piece ^ (row & 7))];
+                f32x4 y = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll
+                for (int k = 1; k < KW; ++k) y += *reinterpret_cast<const f32x4*>(at + k * (ROWS * BN));
+                fwd_epilogue::finish(a.e, added[u], g, m, o, a.n, y);
+            }
+        }
+    }
+}
+
+// k below eight: one output per lane.
+__global__ void __launch_bounds__(256) short_kernel(const Args a) {
+    const int o = blockIdx.x * 256 + threadIdx.x, g = blockIdx.z;
+    if (o >= a.n) return;
+    for (long long m = blockIdx.y; m < a.rows; m += gridDim.y) {
+        float y = 0.0f;
+        for (int i = 0; i < a.k; ++i)
+            y += fwd_epilogue::widen(a.x[g * a.x_gs + m * a.ldx + i]) * fwd_epilogue::widen(a.w[g * a.w_gs + (long long)o * a.ldw + i]);
+        fwd_epilogue::finish(a.e, fwd_epilogue::request(a.e, g, m, o, o + 1), g, m, o, o + 1, f32x4{y, 0.0f, 0.0f, 0.0f});
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- choices
+
+template <int CK, int NT, int T, int KS, bool ANY>
+int32_t stream(const Args& a) {
+    const dim3 grid((unsigned)(((a.n + 15) / 16 + T - 1) / T), (unsigned)((a.rows + 16 * NT - 1) / (16 * NT)), (unsigned)a.groups);
+    fwd_stream::stream_kernel<CK, NT, T, KS, ANY, Finish>
+        <<<grid, 64 * KS, 0, a.stream>>>(a.x, a.ldx, a.x_gs, a.w, a.ldw, a.w_gs, a.rows, a.n, a.k, Finish{a.e, a.n});
+    return (int32_t)hipGetLastError();
+}
+
+// The weight tiles per workgroup: the power of two (at most TMAX) that brings the grid nearest to one workgroup per CU
+// from above.
+template <int CK, int NT, int KS, int TMAX, bool ANY>
+int32_t stream_tiles(const Args& a) {
+    const long long tiles = (long long)((a.n + 15) / 16) * a.groups;
+    if constexpr (TMAX >= 8) if (tiles > 4 * kCus) return stream<CK, NT, 8, KS, ANY>(a);
+    if constexpr (TMAX >= 4) if (tiles > 2 * kCus) return stream<CK, NT, 4, KS, ANY>(a);
+    if constexpr (TMAX >= 2) if (tiles > kCus) return stream<CK, NT, 2, KS, ANY>(a);
+    return stream<CK, NT, 1, KS, ANY>(a);
+}
+
+// The waves per workgroup, which split k: eight where one tile each is at most a workgroup per CU, four otherwise, one
+// where k is short; chunks of 256 where every wave has whole ones.
+template <int NT, int TMAX, bool ANY>
+int32_t stream_split(const Args& a) {
+    const long long tiles = (long long)((a.n + 15) / 16) * a.groups;
+    if (tiles <= kCus && (ANY ? a.k >= 1024 : a.k % 1024 == 0)) {
+        if (!ANY && a.k % 2048 == 0 && (NT == 1 || tiles * NT <= kCus)) return stream<256, 1, 1, 8, ANY>(a);
+        return stream<128, NT, 1, 8, ANY>(a);
+    }
+    if (ANY ? a.k >= 512 : a.k % 512 == 0) {
+        if (!ANY && a.k % 1024 == 0) return stream_tiles<256, NT, 4, 8, ANY>(a);
+        return stream_tiles<128, NT, 4, TMAX, ANY>(a);
+    }
+    return stream_tiles<128, NT, 1, TMAX, ANY>(a);
+}
+
+template <bool ANY>
+int32_t stream_rows(const Args& a) {
+    if (a.rows <= 16) return stream_split<1, 8, ANY>(a);
+    if (a.rows <= 32) return stream_split<2, 4, ANY>(a);
+    return stream_split<4, 4, ANY>(a);
+}
+
+template <int BM, int BN, int WM, int WN, int KW, int BK, int STAGES, bool FAST>
+int32_t tiles(const Args& a) {
+    const long long count = (long long)((a.rows + (long long)BM - 1) / BM) * ((a.n + (long long)BN - 1) / BN);
+    if (count > 0x7fffffff) return kInvalid;
+    tile_kernel<BM, BN, WM, WN, KW, BK, STAGES, FAST>
+        <<<dim3((unsigned)count, 1, (unsigned)a.groups), 64 * WM * WN * KW, 0, a.stream>>>(a);
+    return (int32_t)hipGetLastError();
+}
+
+// The tile of a product of more than 64 rows. Each shape runs a workgroup per CU, and a step of 64 k takes it about the
+// time of the table, larger tiles less per output (fewer bytes through the CU's load path per product, which bounds them)
+// but in whole rounds of 256: the shape whose rounds take least time is launched. Measured with one round, 8192 k:
+// 128 rows -> 4096 29 us with 64 x 32 tiles, 42 with 64 x 64; 400 rows 44 us with 128 x 64, 61 with 128 x 128, 101 with
+// 64 x 32 (four rounds); 1024 rows 71 us with 128 x 128, 110 with 128 x 256; 2048 rows 124 us with 128 x 256, 136 with
+// 128 x 128; 4096 rows 224 us with 256 x 256, 240 with 128 x 256. Rows at any address take 1.7 times as long, all shapes alike.
+enum Shape { k64x32, k64x64, k128x64, k128x128, k128x256, k256x256 };
+Shape shape_of(const Args& a, bool fast) {
+    constexpr struct { int bm, bn; double us; } table[] = {{64, 32, 0.20}, {64, 64, 0.31}, {128, 64, 0.33},
+                                                           {128, 128, 0.53}, {128, 256, 0.93}, {256, 256, 1.70}};
+    int best = 0;
+    double least = 1e300;
+    for (int i = 0; i < (fast ? 6 : 5); ++i) {
+        const double count = (double)((a.rows + (long long)table[i].bm - 1) / table[i].bm) *
+                             (double)((a.n + (long long)table[i].bn - 1) / table[i].bn) * a.groups;
+        const double time = (double)(long long)((count + kCus - 1) / kCus) * table[i].us;
+        if (time < least) least = time, best = i;
+    }
+    return (Shape)best;
+}
+
+int32_t tiled(const Args& a, bool fast) {
+    const Shape shape = shape_of(a, fast);
+    // k a multiple of 128 for the narrow tiles, whose four waves share a step's k, of 64 for the others
+    if (fast && a.k % 128 == 0) {
+        if (shape == k64x32) return tiles<64, 32, 1, 1, 4, 128, 4, true>(a);
+        if (shape == k64x64) return tiles<64, 64, 1, 1, 4, 128, 4, true>(a);
+        if (shape == k128x64) return tiles<128, 64, 2, 1, 4, 128, 3, true>(a);
+    }
+    if (fast && a.k % 64 == 0) {
+        if (shape == k128x128) return tiles<128, 128, 2, 2, 2, 64, 4, true>(a);
+        if (shape == k128x256) return tiles<128, 256, 2, 4, 1, 64, 3, true>(a);
+        if (shape == k256x256) return tiles<256, 256, 2, 4, 1, 32, 4, true>(a);
+    }
+    switch (shape) {
+        case k64x32: return tiles<64, 32, 1, 1, 4, 128, 3, false>(a);
+        case k64x64: return tiles<64, 64, 2, 2, 1, 64, 3, false>(a);
+        case k128x64: return tiles<128, 64, 2, 1, 4, 128, 3, false>(a);
+        case k128x128: return tiles<128, 128, 2, 2, 2, 64, 3, false>(a);
+        default: return tiles<128, 256, 2, 4, 1, 64, 3, false>(a);
+    }
 }
 
 inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -104,16 +389,18 @@ extern "C" int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, in
         !aligned(residual, cell))
         return kInvalid;
     if (residual == out && (ldr != ldo || (groups > 1 && r_gstride != o_gstride))) return kInvalid;
-    const Args a{x, ldx, x_gstride, w, ldw, w_gstride, rows, n, k,
-                 Epilogue{bias, b_gstride, act, residual, ldr, r_gstride, out, out_f32, ldo, o_gstride}};
-    const bool vec = aligned(x, 16) && aligned(w, 16) && ldx % 8 == 0 && ldw % 8 == 0 && x_gstride % 8 == 0 &&
-                     w_gstride % 8 == 0 && k % 8 == 0;
-    const unsigned row_tiles = ((unsigned)rows + 63) / 64, col_tiles = ((unsigned)n + 63) / 64;
-    if (row_tiles > 65535) return kInvalid;
-    const dim3 grid(col_tiles, row_tiles, (unsigned)groups);
-    if (vec)
-        any_kernel<true><<<grid, 256, 0, stream>>>(a);
-    else
-        any_kernel<false><<<grid, 256, 0, stream>>>(a);
-    return (int32_t)hipGetLastError();
+    const Args a{x, ldx, x_gstride, w, ldw, w_gstride, groups, rows, n, k,
+                 Epilogue{bias, b_gstride, act, residual, ldr, r_gstride, out, out_f32, ldo, o_gstride}, stream};
+    if (k < 8) {
+        short_kernel<<<dim3((unsigned)((n + 255LL) / 256), (unsigned)(rows < 1024 ? rows : 1024), (unsigned)groups), 256, 0, stream>>>(a);
+        return (int32_t)hipGetLastError();
+    }
+    const bool fast = aligned(x, 16) && aligned(w, 16) && ldx % 8 == 0 && ldw % 8 == 0 && x_gstride % 8 == 0 &&
+                      w_gstride % 8 == 0;
+    // Up to 64 rows the weights stream past the rows once; with up to 256 too where a workgroup per sixteen outputs and 64 rows is at
+    // most one per CU (200 rows 4096 -> 512: 10 us against 15 with 64 x 32 tiles, which have as few).
+    const long long thin = (long long)((n + 15LL) / 16) * ((rows + 63LL) / 64) * groups;
+    if (rows <= 64 || (rows <= 256 && thin <= kCus))
+        return fast && n % 16 == 0 && k % 128 == 0 ? stream_rows<false>(a) : stream_rows<true>(a);
+    return tiled(a, fast);
 }

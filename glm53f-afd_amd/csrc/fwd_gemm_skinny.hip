@@ -11,26 +11,11 @@
 // not depend on the rows beside it or on their number. No bit-level contract (the reference has none above 8 rows: its own test holds
 // the vendor GEMM to the GEMV within f32 rounding).
 //
-// Shape of the work. A workgroup owns T tiles of sixteen outputs; its KS waves split the K range; a wave walks its
-// range in chunks of CK. Both operands reach the matrix core's fragment layout (lane l: row l % 16, k = 8 (l / 16)
-// .. + 7 of a step of 32) through LDS, because the layout's natural load - sixteen rows of 64 bytes per instruction
-// - asks the texture path for 64 cache lines per KiB: a kernel that loads fragments directly, activations from the
-// L2 in the same way, reaches 2.9 TB/s of weights on 4096 -> 24,640 with sixteen rows, this one 6.4 TB/s. Here
-//   - a load instruction covers whole runs of a row (CK = 256: two rows of 512 consecutive bytes, lanes 0..31 one
-//     row, 32..63 the next; CK = 128: four rows of 256 bytes), CK / 32 of them a tile of sixteen rows x CK; the
-//     wave writes the tile to its own LDS rows (2 CK + 16 bytes apart: a fragment read's sixteen rows then fall on
-//     all 64 banks once) and reads it back as CK / 32 fragments. No workgroup barrier: a wave's LDS instructions
-//     run in order, and the region is its own;
-//   - the activations' tiles (NT of sixteen rows) go the same way once per chunk and stay in registers for the T
-//     weight tiles, so their traffic from the L2 is NT / T of the weight stream;
-//   - two sets of loads alternate over the items of a chunk (the NT activation tiles, then the T weight tiles):
-//     the next item is requested before the current one is waited for.
-// The launch takes T so that the grid is at most one workgroup per CU where the registers allow (measured: one
-// round of 193 workgroups of four waves at T = 8 runs 4096 -> 24,640 in 31.3 us, 385 at T = 4 in 33.6, and 257 at
-// T = 6 - one more than the CUs, so a second round of one - in 40.7).
+// The kernel is stream_kernel of fwd_stream.h; this file chooses its shape.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fwd_stream.h"
 #include "glm53f_fwd_gemv.h"
 
 namespace fwd_gemm {
@@ -39,150 +24,22 @@ namespace {
 constexpr int kInvalid = 1;                       // hipErrorInvalidValue
 constexpr int kCus = 256;
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ uint32_t f2bf2(float lo, float hi) {
-    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    const f2 v = {lo, hi};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf2));
-}
-
-template <int CK> struct Staged {
-    static constexpr int N8 = CK / 32;            // loads of an item = fragments of an item
-    static constexpr int LANES = CK / 8;          // lanes that cover one row's CK elements with 16 bytes each
-    static constexpr int ROW = 2 * CK + 16;       // bytes between a staged tile's rows
-    static constexpr int BYTES = 16 * ROW;        // a wave's staging region
-};
-
-// CK: k per chunk. NT: tiles of sixteen rows (rows <= 16 NT). T: tiles of sixteen outputs per workgroup. KS: waves
-// of a workgroup, each with k / KS of the K range (a multiple of CK).
-template <int CK, int NT, int T, int KS>
-__global__ void __launch_bounds__(64 * KS) stream_kernel(const uint16_t* __restrict__ x, long long ldx, long long x_gs,
-                                                         const uint16_t* __restrict__ w, long long ldw, long long w_gs,
-                                                         int rows, int n, int k, void* __restrict__ out, int out_f32,
-                                                         long long ldo, long long o_gs) {
-    using S = Staged<CK>;
-    constexpr int N8 = S::N8, RPL = 64 / S::LANES, NI = NT + T;
-    constexpr int PART = KS * T * NT * 1024;      // the partial tiles reuse the staging regions
-    constexpr int LDS_BYTES = KS * S::BYTES > PART ? KS * S::BYTES : PART;
-    __shared__ __align__(16) unsigned char lds[LDS_BYTES];
-    const int t = threadIdx.x, lane = t & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int g = blockIdx.z, tiles = n / 16, tile0 = blockIdx.x * T;
-    const int row0 = blockIdx.y * (16 * NT);      // gridDim.y > 1: the rows in groups of 16 NT, a workgroup each
-    rows = min(rows - row0, 16 * NT);
-    const int kc = k / KS, lo = wave * kc, chunks = kc / CK;
-    const int lrow = lane / S::LANES, lcol = 8 * (lane % S::LANES);
-    unsigned char* stage = lds + wave * S::BYTES;
-    unsigned char* put = stage + lrow * S::ROW + 2 * lcol;                        // + RPL j rows
-    const unsigned char* get = stage + (lane & 15) * S::ROW + 16 * (lane >> 4);   // + 64 s
-
-    // items 0 .. NT - 1 of a chunk: the activations' tiles (a row past the end repeats the last one: its column
-    // is not stored); item NT + i: weight tile i of this workgroup (a tile past the last repeats it, not stored)
-    const uint16_t* xsrc = x + g * x_gs + (long long)row0 * ldx + lo + lcol;
-    const uint16_t* wsrc = w + g * w_gs + (long long)lrow * ldw + lo + lcol;
-    auto request = [&](u32x4 (&set)[N8], int item, int c) {
-        if (item < NT) {
-#pragma unroll
-            for (int j = 0; j < N8; ++j)
-                set[j] = *reinterpret_cast<const u32x4*>(xsrc + (long long)min(16 * item + RPL * j + lrow, rows - 1) * ldx + CK * c);
-        } else {
-            const uint16_t* src = wsrc + (long long)(16 * min(tile0 + item - NT, tiles - 1)) * ldw + CK * c;
-#pragma unroll
-            for (int j = 0; j < N8; ++j)
-                set[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + (long long)(RPL * j) * ldw));
-        }
-    };
-    auto fragments = [&](const u32x4 (&set)[N8], u32x4 (&frag)[N8]) {
-#pragma unroll
-        for (int j = 0; j < N8; ++j) *reinterpret_cast<u32x4*>(put + RPL * j * S::ROW) = set[j];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int s = 0; s < N8; ++s) frag[s] = *reinterpret_cast<const u32x4*>(get + 64 * s);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
-
-    f32x4 acc[T][NT];
-#pragma unroll
-    for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[i][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    u32x4 xf[NT][N8];
-
-    // One chunk: `first` holds (or has in flight) the chunk's item 0, the sets alternate from there; the item
-    // after the chunk's last (the next chunk's item 0; after the last chunk a repeat, not used) goes to the set
-    // that the next call names `first`.
-    auto chunk = [&](u32x4 (&first)[N8], u32x4 (&second)[N8], int c) {
-#pragma unroll
-        for (int item = 0; item < NI; ++item) {
-            u32x4 (&cur)[N8] = (item & 1) ? second : first;
-            u32x4 (&nxt)[N8] = (item & 1) ? first : second;
-            if (item + 1 < NI) request(nxt, item + 1, c);
-            else request(nxt, 0, min(c + 1, chunks - 1));
-            if (item < NT) {
-                fragments(cur, xf[item]);
-            } else {
-                u32x4 wf[N8];
-                fragments(cur, wf);
-#pragma unroll
-                for (int s = 0; s < N8; ++s)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        f32x4& a = acc[item - NT][nt];
-                        a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wf[s]),
-                                                                    __builtin_bit_cast(bf16x8, xf[nt][s]), a, 0, 0, 0);
-                    }
-            }
-        }
-    };
-    u32x4 sa[N8], sb[N8];
-    request(sa, 0, 0);
-    if constexpr (NI % 2 == 0) {                  // an even number of items: every chunk starts on the same set
-        for (int c = 0; c < chunks; ++c) chunk(sa, sb, c);
-    } else {
-        int c = 0;
-        for (; c + 1 < chunks; c += 2) {
-            chunk(sa, sb, c);
-            chunk(sb, sa, c + 1);
-        }
-        if (c < chunks) chunk(sa, sb, c);
-    }
-
-    // acc[i][nt][e] = C[output 16 (tile0 + i) + 4 (lane / 16) + e][row 16 nt + lane % 16]: the waves' partial tiles,
-    // added in wave order (the staging regions are free once every wave has left the loop)
-    float* part = reinterpret_cast<float*>(lds);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < T; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-            *reinterpret_cast<f32x4*>(&part[(((wave * T + i) * NT + nt) * 64 + lane) * 4]) = acc[i][nt];
-    __syncthreads();
-    for (int e = t; e < T * NT * 64; e += 64 * KS) {
-        const int tn = e >> 6, l = e & 63, i = tn / NT, nt = tn % NT;
-        f32x4 s = *reinterpret_cast<const f32x4*>(&part[(tn * 64 + l) * 4]);
-#pragma unroll
-        for (int kk = 1; kk < KS; ++kk) {
-            const f32x4 p = *reinterpret_cast<const f32x4*>(&part[((kk * T * NT + tn) * 64 + l) * 4]);
-            s = f32x4{s[0] + p[0], s[1] + p[1], s[2] + p[2], s[3] + p[3]};
-        }
-        const int row = 16 * nt + (l & 15), o = 16 * (tile0 + i) + 4 * (l >> 4);
-        if (row >= rows || tile0 + i >= tiles) continue;
+// The bare product: four outputs as f32, or as bf16 in two accesses.
+struct Plain {
+    void* out;
+    int out_f32;
+    long long ldo, o_gs;
+    __device__ __forceinline__ void operator()(int g, int row, int o, fwd_stream::f32x4 s) const {
         if (out_f32) {
-            float* dst = static_cast<float*>(out) + g * o_gs + (long long)(row0 + row) * ldo + o;
+            float* dst = static_cast<float*>(out) + g * o_gs + (long long)row * ldo + o;
             dst[0] = s[0]; dst[1] = s[1]; dst[2] = s[2]; dst[3] = s[3];
         } else {
-            uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + g * o_gs + (long long)(row0 + row) * ldo + o);
-            dst[0] = f2bf2(s[0], s[1]);
-            dst[1] = f2bf2(s[2], s[3]);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + g * o_gs + (long long)row * ldo + o);
+            dst[0] = fwd_stream::f2bf2(s[0], s[1]);
+            dst[1] = fwd_stream::f2bf2(s[2], s[3]);
         }
     }
-}
+};
 
 struct Args {
     const uint16_t* x; long long ldx, x_gs;
@@ -195,8 +52,8 @@ struct Args {
 template <int CK, int NT, int T, int KS>
 int32_t launch(const Args& a) {
     const dim3 grid((unsigned)((a.n / 16 + T - 1) / T), (unsigned)((a.rows + 16 * NT - 1) / (16 * NT)), (unsigned)a.groups);
-    stream_kernel<CK, NT, T, KS><<<grid, 64 * KS, 0, a.stream>>>(a.x, a.ldx, a.x_gs, a.w, a.ldw, a.w_gs, a.rows, a.n, a.k,
-                                                                 a.out, a.out_f32, a.ldo, a.o_gs);
+    fwd_stream::stream_kernel<CK, NT, T, KS, false, Plain><<<grid, 64 * KS, 0, a.stream>>>(
+        a.x, a.ldx, a.x_gs, a.w, a.ldw, a.w_gs, a.rows, a.n, a.k, Plain{a.out, a.out_f32, a.ldo, a.o_gs});
     return (int32_t)hipGetLastError();
 }
 
