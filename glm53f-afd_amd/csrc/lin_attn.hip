@@ -15,48 +15,40 @@ constexpr int THREADS = 256;
 
 typedef long long ll;
 
-// N consecutive bf16 values, in one access where the address is aligned to all of them.
-template <int N, bool VEC>
+// N consecutive bf16 values of a row, whatever its address: global memory takes vectors at any element.
+template <int N>
 __device__ __forceinline__ void load_row(const bf16_t* p, bf16_t (&e)[N]) {
-    if constexpr (VEC && N >= 8) {
+    if constexpr (N == 1) {
+        e[0] = p[0];
+    } else {
+        constexpr int V = N > 8 ? 8 : N;
+        typedef uint32_t vec __attribute__((ext_vector_type(V / 2), aligned(2)));
 #pragma unroll
-        for (int i = 0; i < N; i += 8) {
-            const kda::u32x4_t x = *reinterpret_cast<const kda::u32x4_t*>(p + i);
+        for (int i = 0; i < N; i += V) {
+            const vec x = *reinterpret_cast<const vec*>(p + i);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < V / 2; ++c) {
                 e[i + 2 * c] = (bf16_t)x[c];
                 e[i + 2 * c + 1] = (bf16_t)(x[c] >> 16);
             }
         }
-    } else if constexpr (VEC && N == 4) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        e[0] = (bf16_t)x.x, e[1] = (bf16_t)(x.x >> 16), e[2] = (bf16_t)x.y, e[3] = (bf16_t)(x.y >> 16);
-    } else if constexpr (VEC && N == 2) {
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(p);
-        e[0] = (bf16_t)x, e[1] = (bf16_t)(x >> 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) e[i] = p[i];
     }
 }
 
-template <int N, bool VEC>
+template <int N>
 __device__ __forceinline__ void store_row(bf16_t* p, const float (&x)[N]) {
-    if constexpr (VEC && N >= 2) {
-        uint32_t w[N / 2];
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) w[i] = kda::f2bf2(x[2 * i], x[2 * i + 1]);
-        if constexpr (N >= 8) {
-#pragma unroll
-            for (int i = 0; i < N / 2; i += 4) *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        } else if constexpr (N == 4) {
-            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-        } else {
-            *reinterpret_cast<uint32_t*>(p) = w[0];
-        }
+    if constexpr (N == 1) {
+        p[0] = kda::f2bf(x[0]);
     } else {
+        constexpr int V = N > 8 ? 8 : N;
+        typedef uint32_t vec __attribute__((ext_vector_type(V / 2), aligned(2)));
 #pragma unroll
-        for (int i = 0; i < N; ++i) p[i] = kda::f2bf(x[i]);
+        for (int i = 0; i < N; i += V) {
+            vec w;
+#pragma unroll
+            for (int c = 0; c < V / 2; ++c) w[c] = kda::f2bf2(x[i + 2 * c], x[i + 2 * c + 1]);
+            *reinterpret_cast<vec*>(p + i) = w;
+        }
     }
 }
 
@@ -98,7 +90,7 @@ struct ChainArgs {
 // holds ST consecutive value rows, so that its values and its outputs are one access each. Value rows do not meet, so the
 // cut changes no bit; small batches take the finer one to reach more CUs. The product of two bf16 values is exact in f32,
 // so the update has one rounding of the decayed state and one of the sum.
-template <typename S, int DK, int NROW, bool READ, bool VEC>
+template <typename S, int DK, int NROW, bool READ>
 __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
     constexpr int KPL = kda::StateGeo<S>::KPL, LPR = DK / KPL, GROUPS = THREADS / LPR, ST = NROW / GROUPS;
     static_assert(ST >= 1, "a lane holds a value row at least");
@@ -119,9 +111,9 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 
     bf16_t kn[KPL], qn[KPL], vn[ST];              // the next row's pieces
     if (rows > 0) {
-        load_row<KPL, VEC>(k, kn);
-        if constexpr (READ) load_row<KPL, VEC>(q, qn);
-        load_row<ST, VEC>(v, vn);
+        load_row<KPL>(k, kn);
+        if constexpr (READ) load_row<KPL>(q, qn);
+        load_row<ST>(v, vn);
     }
     const float fade = expf(a.log_decay[lh]);
     uint4 raw[ST];
@@ -142,9 +134,9 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 #pragma unroll
         for (int j = 0; j < ST; ++j) vv[j] = kda::bf2f(vn[j]);
         if (t + 1 < rows) {
-            load_row<KPL, VEC>(k + (t + 1) * a.k_stride, kn);
-            if constexpr (READ) load_row<KPL, VEC>(q + (t + 1) * a.q_stride, qn);
-            load_row<ST, VEC>(v + (t + 1) * a.v_stride, vn);
+            load_row<KPL>(k + (t + 1) * a.k_stride, kn);
+            if constexpr (READ) load_row<KPL>(q + (t + 1) * a.q_stride, qn);
+            load_row<ST>(v + (t + 1) * a.v_stride, vn);
         }
         float o[ST];
 #pragma unroll
@@ -159,7 +151,7 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
         }
         if constexpr (READ) {
             if (threadIdx.x % LPR == 0)
-                store_row<ST, VEC>(a.out + (row0 + (ll)t) * a.out_stride + (ll)h * a.dv + val0, o);
+                store_row<ST>(a.out + (row0 + (ll)t) * a.out_stride + (ll)h * a.dv + val0, o);
         }
     }
     if (a.state_out == nullptr) return;
@@ -179,11 +171,11 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // of their terms). No power of e^g above 1 is formed, so no decay is too fast.
 //
 // A workgroup is one head of one request over one segment of its rows; wave w holds the state's value rows 32 w .. 32 w + 31
-// in accumulators, s[t][x]: keys 16 t + 4 (lane / 16) + e, value row 32 w + 2 (lane % 16) + x. That order is free, and
-// this one makes a lane's loads of v (two neighbouring columns of eight rows) the operand of the products as it is,
-// without LDS, its state tiles two operands of the read-out, and its outputs eight consecutive values. q and k pass through
-// LDS once per chunk for all waves: as rows for the scores (keys in the order that the state's accumulators have), and k
-// transposed for the state, from the same registers.
+// in accumulators, 32 keys x 32 values of it per lane and four tiles. The rows of q, k and v go from memory straight to LDS,
+// a chunk ahead, and are read from there in both directions: whole 16-byte pieces of sixteen rows (scores, read-out), and
+// transposed, four rows of a column per lane (what the state adds, and the values of the read-out). The order of keys in the
+// state's tiles and of values over the lanes is free; it is the one that makes a lane's two state tiles eight consecutive keys
+// of one value row, so that they are an operand of the read-out as they stand, and its outputs eight consecutive values.
 //
 // Few requests leave most CUs idle for a long prompt, so the rows are cut into segments: segment_kernel (SUMS) forms what
 // each segment adds to a state, starts_kernel runs over them to the state at every segment's start, and the outputs of
@@ -194,6 +186,8 @@ constexpr int C = 32;                             // rows per chunk: one product
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));   // at any element's address
 
 template <typename S>
 struct PrefillArgs {
@@ -219,7 +213,6 @@ struct PrefillArgs {
 // e^{g n}; 1 for n = 0 also where nothing is remembered (g = -inf).
 __device__ __forceinline__ float fade_of(float g, int n) { return n == 0 ? 1.0f : expf(g * (float)n); }
 
-__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 
 __device__ __forceinline__ bf16x8 operand(const uint32_t (&w)[4]) {
@@ -230,61 +223,70 @@ __device__ __forceinline__ bf16x8 operand(const bf16_t* lds) {
     return __builtin_bit_cast(bf16x8, *reinterpret_cast<const kda::u32x4_t*>(lds));
 }
 
+// Two of a transposed read: the sixteen lanes of a group name four rows of sixteen values, four lanes of 8 bytes a row, and
+// each gets one column of the four rows.
+__device__ __forceinline__ void column(const bf16_t* lds, uint32_t* w) {
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds);
+    w[0] = (uint16_t)x[0] | (uint32_t)(uint16_t)x[1] << 16;
+    w[1] = (uint16_t)x[2] | (uint32_t)(uint16_t)x[3] << 16;
+}
+
 __device__ __forceinline__ f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight f32 values as hi + lo: hi their upper halves, lo the rest rounded to bf16.
-__device__ __forceinline__ void two_terms(const float (&x)[8], bf16x8& hi, bf16x8& lo) {
-    uint32_t h[4], l[4];
+// N f32 values as hi + lo: hi their upper halves, lo the rest rounded to bf16; two values to a word.
+template <int N>
+__device__ __forceinline__ void two_terms(const float (&x)[N], uint32_t (&hi)[N / 2], uint32_t (&lo)[N / 2]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N / 2; ++i) {
         const uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
-        h[i] = high_halves(a, b);
-        l[i] = kda::f2bf2(x[2 * i] - __uint_as_float(a & 0xffff0000u), x[2 * i + 1] - __uint_as_float(b & 0xffff0000u));
+        hi[i] = high_halves(a, b);
+        lo[i] = kda::f2bf2(x[2 * i] - __uint_as_float(a & 0xffff0000u), x[2 * i + 1] - __uint_as_float(b & 0xffff0000u));
     }
-    hi = operand(h), lo = operand(l);
 }
 
-// Two neighbouring elements of a row; FAST: in one access (the rows are 4-byte aligned).
-template <bool FAST>
-__device__ __forceinline__ uint32_t load_pair(const bf16_t* p) {
-    if constexpr (FAST) return *reinterpret_cast<const uint32_t*>(p);
-    return p[0] | ((uint32_t)p[1] << 16);
+// Where the 16-byte pieces of an LDS row stand: at piece ^ turn(row). Chosen for the two ways of reading: sixteen rows at one
+// piece (a group of lanes that LDS serves at a time then meets every bank once), and four consecutive rows at four consecutive
+// pieces. PIECES: of a row, 16, 8 or 4.
+template <int PIECES>
+__device__ __forceinline__ int turn(int row) {
+    const int low = ((row >> 2 & 1) << 1) ^ ((row >> 3 & 1) * 3);
+    if constexpr (PIECES == 16) return (row & 3) << 2 | low;
+    if constexpr (PIECES == 8) return (row >> 1 & 1) << 2 | low;
+    return low;
 }
+
+// 16 bytes per lane from global memory to LDS without a register in between: to lds + 16 lane (lds the same in all lanes). Written
+// out because the compiler, which cannot tell the buffers apart, has every read of one wait for the loads of the other;
+// who reads waits himself, before a barrier.
+__device__ __forceinline__ void to_lds(const bf16_t* src, bf16_t* lds) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) bf16_t*)lds);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(at) : "memory");
+}
+
+// Key and value of element e of a lane's tile (t, x) of its wave's state: eight consecutive keys from tiles t, t + 1 (t even).
+__device__ __forceinline__ int key_of(int t, int grp) { return 32 * (t / 2) + 8 * grp + 4 * (t & 1); }
+__device__ __forceinline__ int value_of(int x, int wave, int col) { return 32 * wave + 8 * (col >> 2) + 4 * x + (col & 3); }
 
 // A wave's part of a state in memory ([value][key]) and its accumulators.
 template <typename S, int DK>
-__device__ __forceinline__ void load_state(const S* p, f32x4 (&s)[DK / 16][2]) {
+__device__ __forceinline__ f32x4 load_tile(const S* p, int t, int x) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            const S* at = p + (32 * wave + 2 * (lane & 15) + x) * DK + 16 * t + 4 * (lane >> 4);
-            if constexpr (sizeof(S) == 4) {
-                s[t][x] = *reinterpret_cast<const f32x4*>(at);
-            } else {
-                const uint2 w = *reinterpret_cast<const uint2*>(at);
-                s[t][x] = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                                __uint_as_float(w.y & 0xffff0000u)};
-            }
-        }
+    const S* at = p + value_of(x, wave, lane & 15) * DK + key_of(t, lane >> 4);
+    if constexpr (sizeof(S) == 4) return *reinterpret_cast<const f32x4*>(at);
+    const uint2 w = *reinterpret_cast<const uint2*>(at);
+    return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                 __uint_as_float(w.y & 0xffff0000u)};
 }
 template <typename S, int DK>
-__device__ __forceinline__ void store_state(S* p, const f32x4 (&s)[DK / 16][2]) {
+__device__ __forceinline__ void store_tile(S* p, int t, int x, f32x4 v) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            S* at = p + (32 * wave + 2 * (lane & 15) + x) * DK + 16 * t + 4 * (lane >> 4);
-            const f32x4 v = s[t][x];
-            if constexpr (sizeof(S) == 4)
-                *reinterpret_cast<f32x4*>(at) = v;
-            else
-                *reinterpret_cast<uint2*>(at) = make_uint2(kda::f2bf2(v[0], v[1]), kda::f2bf2(v[2], v[3]));
-        }
+    S* at = p + value_of(x, wave, lane & 15) * DK + key_of(t, lane >> 4);
+    if constexpr (sizeof(S) == 4)
+        *reinterpret_cast<f32x4*>(at) = v;
+    else
+        *reinterpret_cast<uint2*>(at) = make_uint2(kda::f2bf2(v[0], v[1]), kda::f2bf2(v[2], v[3]));
 }
 
 // The same part in the workspace: a lane's accumulators 16 bytes each, a wave's instruction 1 KiB.
@@ -294,16 +296,19 @@ __device__ __forceinline__ float* work_at(float* work, ll index) {
 }
 
 // SUMS: what the segment adds to a state, into the workspace; otherwise its outputs, and behind a request's last row
-// the state. FAST: q, k and v rows are 4-byte aligned and out rows 16-byte aligned.
+// the state. FAST: the rows of q, k and v are 16-byte aligned and go straight to LDS; otherwise through registers.
 template <typename S, int DK, int NW, bool FAST, bool SUMS>
-__global__ void __launch_bounds__(64 * NW, NW / 2) segment_kernel(const PrefillArgs<S> a) {
-    constexpr int T = 64 * NW, KT = DK / 16, PITCH = DK + 8, DV = 32 * NW;
-    constexpr int TERMS = 3;
-    constexpr int ITEMS = SUMS ? (2 * DK + T - 1) / T : 4 * DK / T;   // (eight rows, two columns) of k, then of q, per thread
-    __shared__ __align__(16) bf16_t ks[SUMS ? 1 : C * PITCH], qs[SUMS ? 1 : C * PITCH], kt[DK * C], ph[SUMS ? 1 : C * C],
-        pl[SUMS ? 1 : C * C];
+__global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kernel(const PrefillArgs<S> a) {
+    constexpr int T = 64 * NW, KT = DK / 16, DV = 32 * NW, TERMS = 3;
+    constexpr int KP = DK / 8, VP = DV / 8;                          // pieces of a row
+    constexpr int QN = SUMS ? 0 : C * KP / T, KN = C * KP / T, VN = C * VP / T, N = QN + KN + VN;   // pieces per thread and chunk
+    static_assert(C * KP % T == 0 && C * VP % T == 0, "whole pieces");
+    constexpr int SET = (SUMS ? 1 : 2) * C * DK + C * DV;            // a chunk's rows in LDS: k, v, q
+    __shared__ __align__(16) bf16_t lds[2 * SET + (SUMS ? 0 : 2 * C * C)];
+    bf16_t* ph = lds + 2 * SET;                                      // the scores' terms [row][column]
+    bf16_t* pl = ph + C * C;
     const int h = blockIdx.x % a.heads, seg = blockIdx.x / a.heads, b = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), col = lane & 15, grp = lane >> 4;
     const int first = a.cu_rows[b], rows = max(min(a.cu_rows[b + 1] - first, a.most), 0);
     const int begin = seg * a.seg_rows;
     if (begin >= rows && (seg > 0 || SUMS)) return;
@@ -315,146 +320,116 @@ __global__ void __launch_bounds__(64 * NW, NW / 2) segment_kernel(const PrefillA
     const float g = a.log_decay[h];
     const ll row0 = (ll)first + begin, hk = h / a.group;
 
-    // what this thread moves of k and q: rows 8 oct .., columns 2 c2 and 2 c2 + 1
-    const bf16_t* src[ITEMS];
-    ll step[ITEMS];
-    int oct[ITEMS], c2[ITEMS];
-    bool is_k[ITEMS], on[ITEMS];
+    // Piece i of this thread: LDS slot t + T i of k's rows, then v's, then q's; row slot / pieces of a row. A row past the segment's
+    // last repeats it.
+    auto place_of = [&](int i) { return i < KN ? i * T * 8 : i < KN + VN ? C * DK + (i - KN) * T * 8 : C * (DK + DV) + (i - KN - VN) * T * 8; };
+    u32x4_any held[FAST ? 1 : N];
+    auto request = [&](int c, bf16_t* set) {
 #pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
-        const int id = it * T + threadIdx.x;
-        is_k[it] = SUMS || id < 2 * DK;
-        on[it] = !SUMS || id < 2 * DK;
-        oct[it] = (id / (DK / 2)) & 3;
-        c2[it] = id % (DK / 2);
-        step[it] = is_k[it] ? a.k_stride : a.q_stride;
-        src[it] = (is_k[it] ? a.k : a.q) + (row0 + 8 * oct[it]) * step[it] + hk * DK + 2 * c2[it];
-    }
-    const bf16_t* vsrc = a.v + (row0 + 8 * grp) * a.v_stride + (ll)h * DV + 32 * wave + 2 * col;
-
-    uint32_t raw[ITEMS][8], vraw[8];
-    auto load = [&](int c) {
-        const int live = n - c * C;               // rows of the request that the chunk holds; the others are zeros
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                raw[it][e] = on[it] && 8 * oct[it] + e < live ? load_pair<FAST>(src[it] + (c * C + e) * step[it]) : 0u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vraw[e] = 8 * grp + e < live ? load_pair<FAST>(vsrc + (c * C + e) * a.v_stride) : 0u;
+        for (int i = 0; i < N; ++i) {
+            const bool is_v = i >= KN && i < KN + VN;
+            const int pieces = is_v ? VP : KP, slot = t + T * (i < KN ? i : is_v ? i - KN : i - KN - VN);
+            const int row = slot / pieces, piece = (slot % pieces) ^ (is_v ? turn<VP>(row) : turn<KP>(row));
+            const ll r = row0 + min(c * C + row, n - 1);
+            const bf16_t* src = i < KN ? a.k + r * a.k_stride + hk * DK : is_v ? a.v + r * a.v_stride + (ll)h * DV : a.q + r * a.q_stride + hk * DK;
+            if constexpr (FAST) to_lds(src + 8 * piece, set + place_of(i) + wave * 512);
+            else held[i] = *reinterpret_cast<const u32x4_any*>(src + 8 * piece);
+        }
     };
+    auto place = [&](bf16_t* set) {               // the registers' pieces
+        if constexpr (!FAST) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) *reinterpret_cast<kda::u32x4_t*>(set + place_of(i) + t * 8) = held[i];
+        }
+    };
+    if (n > 0) request(0, lds);
 
     f32x4 s[KT][2];
     if constexpr (SUMS) {
 #pragma unroll
-        for (int t = 0; t < KT; ++t) s[t][0] = s[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int m = 0; m < KT; ++m) s[m][0] = s[m][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     } else if (a.work) {
         const float* w = work_at<DK, NW>(a.work, ((ll)b * a.heads + h) * a.segs + seg);
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) s[t][x] = *reinterpret_cast<const f32x4*>(w + (2 * t + x) * 256);
+            for (int x = 0; x < 2; ++x) s[m][x] = *reinterpret_cast<const f32x4*>(w + (2 * m + x) * 256);
     } else {
-        load_state<S, DK>(a.state_in + state_at, s);
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) s[m][x] = load_tile<S, DK>(a.state_in + state_at, m, x);
     }
 
-    // the decays of a whole chunk that this lane uses
+    // The decays of a whole chunk that this lane uses: of its rows of v to the chunk's end, of the chunk's start to its two
+    // rows of outputs, and between the rows of its scores. The score tiles (rows, columns) on and below the diagonal are
+    // (0, 0), (1, 0), (1, 1), tile m for wave m mod NW: a wave has tiles of one kind.
     float in_tail[8], to_row[2], between[4];
-    const int tiles_i[3] = {0, 1, 1}, tiles_j[3] = {0, 0, 1};         // the score tiles on and below the diagonal
-    if (n > 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) in_tail[e] = fade_of(g, C - 1 - (8 * grp + e));
-        if constexpr (!SUMS) {
+    for (int e = 0; e < 8; ++e) in_tail[e] = fade_of(g, C - 1 - (8 * grp + e));
+    if constexpr (!SUMS) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) to_row[i] = fade_of(g, 16 * i + col + 1);
-            for (int i = threadIdx.x; i < C * C / 2; i += T)
-                reinterpret_cast<uint32_t*>(ph)[i] = reinterpret_cast<uint32_t*>(pl)[i] = 0u;   // the tile above the diagonal
+        for (int i = 0; i < 2; ++i) to_row[i] = a.scale * fade_of(g, 16 * i + col + 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int gap = (wave == 1 ? 16 : 0) + col - (4 * grp + e);
+            between[e] = gap < 0 ? 0.0f : a.scale * fade_of(g, gap);
         }
-        load(0);
+        for (int i = t; i < C * C / 2; i += T)                       // the tile above the diagonal
+            reinterpret_cast<uint32_t*>(ph)[i] = reinterpret_cast<uint32_t*>(pl)[i] = 0u;
     }
     const float whole = fade_of(g, C);
-    (void)between;
 
-    for (int c = 0; c * C < n; ++c) {
+    // a lane's places in a set: rows col and 16 + col at piece grp (+ 4 u: 32 elements further, under the turn), and transposed rows
+    // 8 grp + col / 4 and four below at piece col mod 4
+    const int at_row = col * DK + 8 * (grp ^ turn<KP>(col)), at_row16 = (16 + col) * DK + 8 * (grp ^ turn<KP>(16 + col));
+    const int tr0 = 8 * grp + (col >> 2), tr1 = tr0 + 4, j = col & 3;
+    const int at_k0 = tr0 * DK + 8 * (j ^ turn<KP>(tr0)), at_k1 = tr1 * DK + 8 * (j ^ turn<KP>(tr1));
+    const int at_v0 = C * DK + tr0 * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr0)), at_v1 = C * DK + tr1 * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr1));
+
+    int set = 0;
+    for (int c = 0; c * C < n; ++c, set = SET - set) {
         const int live = min(n - c * C, C);
-        // q and k to LDS
+        bf16_t* now = lds + set;
+        const bf16_t* qs = now + C * (DK + DV);
+        // this thread's part of the chunk is there; behind the barrier everybody's is, and the other set is free
+        if constexpr (FAST) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else place(now);
+        __syncthreads();
+        if ((c + 1) * C < n) request(c + 1, lds + (SET - set));
+
+        // v as an operand: two words of four rows, twice, for each half of the wave's values
+        uint32_t vp[2][4];
 #pragma unroll
-        for (int it = 0; it < ITEMS; ++it) {
-            if (!on[it]) continue;
-            if constexpr (!SUMS) {
-                // a row's keys in the order 0-3, 16-19, 4-7, 20-23, .. of every 32: what a lane's two state tiles hold
-                const int piece = (c2[it] & 15) >> 1, at = (c2[it] & ~15) + ((piece & 3) * 2 + (piece >> 2)) * 2 + (c2[it] & 1);
-                uint32_t* dst = reinterpret_cast<uint32_t*>((is_k[it] ? ks : qs) + 8 * oct[it] * PITCH) + at;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) dst[e * (PITCH / 2)] = raw[it][e];
-            }
-            if (is_k[it]) {
-                bf16_t* dst = kt + 2 * c2[it] * C + 8 * (oct[it] ^ (c2[it] & 3));
-                uint32_t w[4];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) w[m] = low_halves(raw[it][2 * m], raw[it][2 * m + 1]);
-                *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-                for (int m = 0; m < 4; ++m) w[m] = high_halves(raw[it][2 * m], raw[it][2 * m + 1]);
-                *reinterpret_cast<uint4*>(dst + C) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+        for (int x = 0; x < 2; ++x) {
+            column(now + at_v0 + 4 * x, &vp[x][0]);
+            column(now + at_v1 + 4 * x, &vp[x][2]);
         }
-        // v as operands: itself, and decayed to the chunk's end in terms
-        uint32_t vp[2][4], vd[TERMS][2][4];
-        {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = live == C ? in_tail[e] : fade_of(g, max(live - 1 - (8 * grp + e), 0));
+        if (live < C) {                           // rows past the last count as zeros
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                vp[0][m] = low_halves(vraw[2 * m], vraw[2 * m + 1]);
-                vp[1][m] = high_halves(vraw[2 * m], vraw[2 * m + 1]);
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    uint32_t part[TERMS][2];
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const uint32_t r = vraw[2 * m + y];
-                        float z = f[2 * m + y] * __uint_as_float(x ? r & 0xffff0000u : r << 16);
-#pragma unroll
-                        for (int i = 0; i < TERMS; ++i) {
-                            part[i][y] = __float_as_uint(z);
-                            z -= __uint_as_float(part[i][y] & 0xffff0000u);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < TERMS; ++i) vd[i][x][m] = high_halves(part[i][0], part[i][1]);
-                }
+                const int r = 8 * grp + 2 * m;
+                const uint32_t keep = (r < live ? 0x0000ffffu : 0u) | (r + 1 < live ? 0xffff0000u : 0u);
+                vp[0][m] &= keep, vp[1][m] &= keep;
             }
         }
-        __syncthreads();
-        if ((c + 1) * C < n) load(c + 1);
-
         if constexpr (!SUMS) {
-            // scores: tile (i, j) with key rows as the first operand, so that a lane holds four consecutive j of a row i
+            // scores: key rows as the first operand, so that a lane holds four consecutive columns of a row
 #pragma unroll
-            for (int tt = 0; tt < 3; ++tt) {
-                if (tt % NW != wave) continue;
-                const int ti = tiles_i[tt], tj = tiles_j[tt];
+            for (int m = 0; m < 3; ++m) {
+                if (m % NW != wave) continue;
+                constexpr int tiles_i[3] = {0, 1, 1}, tiles_j[3] = {0, 0, 1};
+                const int ti = tiles_i[m], tj = tiles_j[m];
                 f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int u = 0; u < DK / 32; ++u)
-                    p = product(operand(ks + (16 * tj + col) * PITCH + 32 * u + 8 * grp), operand(qs + (16 * ti + col) * PITCH + 32 * u + 8 * grp), p);
-                const int i = 16 * ti + col, j = 16 * tj + 4 * grp;
+                    p = product(operand(now + ((tj ? at_row16 : at_row) ^ (32 * u))), operand(qs + ((ti ? at_row16 : at_row) ^ (32 * u))), p);
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = between[e] == 0.0f ? 0.0f : p[e] * between[e];
                 uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    float y[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int gap = i - (j + 2 * m + e);
-                        y[e] = gap < 0 ? 0.0f : p[2 * m + e] * fade_of(g, gap);
-                    }
-                    const uint32_t r0 = __float_as_uint(y[0]), r1 = __float_as_uint(y[1]);
-                    hi[m] = high_halves(r0, r1);
-                    lo[m] = kda::f2bf2(y[0] - __uint_as_float(r0 & 0xffff0000u), y[1] - __uint_as_float(r1 & 0xffff0000u));
-                }
-                const int at = i * C + 8 * ((j >> 3) ^ ((i >> 1) & 3)) + (j & 7);
+                two_terms(y, hi, lo);
+                const int i = 16 * ti + col, jj = 16 * tj + 4 * grp, at = i * C + 8 * ((jj >> 3) ^ turn<4>(i)) + (jj & 7);
                 *reinterpret_cast<uint2*>(ph + at) = make_uint2(hi[0], hi[1]);
                 *reinterpret_cast<uint2*>(pl + at) = make_uint2(lo[0], lo[1]);
             }
@@ -462,27 +437,24 @@ __global__ void __launch_bounds__(64 * NW, NW / 2) segment_kernel(const PrefillA
             f32x4 o[2][2] = {};
 #pragma unroll
             for (int u = 0; u < DK / 32; ++u) {
-                bf16x8 qf[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) qf[i] = operand(qs + (16 * i + col) * PITCH + 32 * u + 8 * grp);
+                const bf16x8 q0 = operand(qs + (at_row ^ (32 * u))), q1 = operand(qs + (at_row16 ^ (32 * u)));
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     float z[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[e] = s[2 * u][x][e], z[4 + e] = s[2 * u + 1][x][e];
-                    bf16x8 hi, lo;
+                    uint32_t hi[4], lo[4];
                     two_terms(z, hi, lo);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        o[x][i] = product(hi, qf[i], o[x][i]);
-                        o[x][i] = product(lo, qf[i], o[x][i]);
-                    }
+                    o[x][0] = product(operand(hi), q0, o[x][0]);
+                    o[x][1] = product(operand(hi), q1, o[x][1]);
+                    o[x][0] = product(operand(lo), q0, o[x][0]);
+                    o[x][1] = product(operand(lo), q1, o[x][1]);
                 }
             }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int at = (16 * i + col) * C + 8 * (grp ^ ((col >> 1) & 3));
+                const int at = (16 * i + col) * C + 8 * (grp ^ turn<4>(16 * i + col));
                 const bf16x8 hi = operand(ph + at), lo = operand(pl + at);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -492,37 +464,63 @@ __global__ void __launch_bounds__(64 * NW, NW / 2) segment_kernel(const PrefillA
                     o[x][i] = product(operand(vp[x]), lo, o[x][i]);
                 }
                 if (16 * i + col < live) {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[2 * e] = o[0][i][e] * a.scale, y[2 * e + 1] = o[1][i][e] * a.scale;
-                    store_row<8, FAST>(a.out + (row0 + c * C + 16 * i + col) * a.out_stride + (ll)h * DV + 32 * wave + 8 * grp, y);
+                    const float y[8] = {o[0][i][0], o[0][i][1], o[0][i][2], o[0][i][3], o[1][i][0], o[1][i][1], o[1][i][2], o[1][i][3]};
+                    store_row<8>(a.out + (row0 + c * C + 16 * i + col) * a.out_stride + (ll)h * DV + 32 * wave + 8 * grp, y);
                 }
             }
+            if (a.state_out == nullptr && last && (c + 1) * C >= n) break;   // nobody reads the state behind the last rows
+        }
+        // v decayed to the chunk's end, in terms
+        uint32_t vd[TERMS][2][4];
+        {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = in_tail[e];
+            if (live < C) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = fade_of(g, max(live - 1 - (8 * grp + e), 0));
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float z0 = f[2 * m] * __uint_as_float(vp[x][m] << 16), z1 = f[2 * m + 1] * __uint_as_float(vp[x][m] & 0xffff0000u);
+#pragma unroll
+                    for (int i = 0; i < TERMS; ++i) {
+                        const uint32_t r0 = __float_as_uint(z0), r1 = __float_as_uint(z1);
+                        vd[i][x][m] = high_halves(r0, r1);
+                        if (i + 1 < TERMS) z0 -= __uint_as_float(r0 & 0xffff0000u), z1 -= __uint_as_float(r1 & 0xffff0000u);
+                    }
+                }
         }
         // the state behind the chunk
         const float by = live == C ? whole : fade_of(g, live);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            const bf16x8 kf = operand(kt + (16 * t + col) * C + 8 * (grp ^ ((col >> 1) & 3)));
+        for (int m = 0; m < KT; ++m) {
+            uint32_t kf[4];
+            column(now + (at_k0 ^ (32 * (m / 2))) + 4 * (m & 1), &kf[0]);
+            column(now + (at_k1 ^ (32 * (m / 2))) + 4 * (m & 1), &kf[2]);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[t][x][e] *= by;
+                for (int e = 0; e < 4; ++e) s[m][x][e] *= by;
 #pragma unroll
-                for (int i = 0; i < TERMS; ++i) s[t][x] = product(kf, operand(vd[i][x]), s[t][x]);
+                for (int i = 0; i < TERMS; ++i) s[m][x] = product(operand(kf), operand(vd[i][x]), s[m][x]);
             }
         }
-        __syncthreads();
     }
 
     if constexpr (SUMS) {
         float* w = work_at<DK, NW>(a.work, ((ll)b * a.heads + h) * a.segs + seg + 1);
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int m = 0; m < KT; ++m)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) *reinterpret_cast<f32x4*>(w + (2 * t + x) * 256) = s[t][x];
+            for (int x = 0; x < 2; ++x) *reinterpret_cast<f32x4*>(w + (2 * m + x) * 256) = s[m][x];
     } else if (last && a.state_out) {
-        store_state<S, DK>(a.state_out + state_at, s);
+#pragma unroll
+        for (int m = 0; m < KT; ++m)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) store_tile<S, DK>(a.state_out + state_at, m, x, s[m][x]);
     }
 }
 
@@ -530,24 +528,25 @@ __global__ void __launch_bounds__(64 * NW, NW / 2) segment_kernel(const PrefillA
 template <typename S, int DK, int NW>
 __global__ void __launch_bounds__(64 * NW) starts_kernel(const PrefillArgs<S> a) {
     const int h = blockIdx.x, b = blockIdx.y, t = blockIdx.z / 2, x = blockIdx.z % 2;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int rows = max(min(a.cu_rows[b + 1] - a.cu_rows[b], a.most), 0);
     const float by = fade_of(a.log_decay[h], a.seg_rows);
-    const S* p = a.state_in + a.state_off[b] + (ll)h * (32 * NW * DK) + (32 * wave + 2 * (lane & 15) + x) * DK + 16 * t + 4 * (lane >> 4);
-    f32x4 s;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(S) == 4) s[e] = p[e];
-        else s[e] = kda::bf2f(p[e]);
-    }
+    f32x4 s = load_tile<S, DK>(a.state_in + a.state_off[b] + (ll)h * (32 * NW * DK), t, x);
     float* w = work_at<DK, NW>(a.work, ((ll)b * a.heads + h) * a.segs) + (2 * t + x) * 256;
     *reinterpret_cast<f32x4*>(w) = s;
-    for (int seg = 1; seg * a.seg_rows < rows; ++seg) {
-        w += 32 * NW * DK;
-        const f32x4 d = *reinterpret_cast<const f32x4*>(w);
+    constexpr int AHEAD = 8;                      // segments requested at a time
+    const int count = (int)(((ll)rows + a.seg_rows - 1) / a.seg_rows);
+    for (int seg0 = 1; seg0 < count; seg0 += AHEAD) {
+        f32x4 d[AHEAD];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(by, s[e], d[e]);
-        *reinterpret_cast<f32x4*>(w) = s;
+        for (int i = 0; i < AHEAD; ++i)
+            if (seg0 + i < count) d[i] = *reinterpret_cast<const f32x4*>(w + (ll)(seg0 + i) * (32 * NW * DK));
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (seg0 + i >= count) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = __builtin_fmaf(by, s[e], d[i][e]);
+            *reinterpret_cast<f32x4*>(w + (ll)(seg0 + i) * (32 * NW * DK)) = s;
+        }
     }
 }
 
@@ -559,29 +558,18 @@ bool good_shape(int heads, int qk_heads, int dk, int dv, int batch) {
            (dv == 64 || dv == 128) && batch >= 1 && batch <= 65535;
 }
 
-// 16-byte accesses of a row buffer: its base and every row.
-inline bool fast_rows(const void* p, ll stride) { return aligned(p, 16) && stride % 8 == 0; }
-
 template <typename S, int DK, int NROW, bool READ>
-int launch_chain(const ChainArgs<S>& a, int layers, int batch, bool vec, hipStream_t stream) {
+int launch_chain(const ChainArgs<S>& a, int layers, int batch, hipStream_t stream) {
     const dim3 grid((unsigned)((ll)layers * a.heads * (a.dv / NROW)), (unsigned)batch);
-    if (vec)
-        chain_kernel<S, DK, NROW, READ, true><<<grid, THREADS, 0, stream>>>(a);
-    else
-        chain_kernel<S, DK, NROW, READ, false><<<grid, THREADS, 0, stream>>>(a);
+    chain_kernel<S, DK, NROW, READ><<<grid, THREADS, 0, stream>>>(a);
     return launched();
 }
 
 template <typename S, bool READ>
 int launch_chain(const ChainArgs<S>& a, int dk, int layers, int batch, hipStream_t stream) {
-    const bool vec = fast_rows(a.k, a.k_stride) && a.k_layer % 8 == 0 && fast_rows(a.v, a.v_stride) && a.v_layer % 8 == 0 &&
-                     (!READ || (fast_rows(a.q, a.q_stride) && fast_rows(a.out, a.out_stride)));
     const bool fine = (ll)layers * a.heads * batch * (a.dv / 64) < 512;   // fewer than two workgroups per CU
-    if (dk == 64)
-        return fine ? launch_chain<S, 64, 32, READ>(a, layers, batch, vec, stream)
-                    : launch_chain<S, 64, 64, READ>(a, layers, batch, vec, stream);
-    return fine ? launch_chain<S, 128, 32, READ>(a, layers, batch, vec, stream)
-                : launch_chain<S, 128, 64, READ>(a, layers, batch, vec, stream);
+    if (dk == 64) return fine ? launch_chain<S, 64, 32, READ>(a, layers, batch, stream) : launch_chain<S, 64, 64, READ>(a, layers, batch, stream);
+    return fine ? launch_chain<S, 128, 32, READ>(a, layers, batch, stream) : launch_chain<S, 128, 64, READ>(a, layers, batch, stream);
 }
 
 // What the chain and the prefill check alike.
@@ -604,21 +592,17 @@ int chain(int heads, int qk_heads, int dk, int dv, int batch, ChainArgs<S> a, hi
     return launch_chain<S, true>(a, dk, 1, batch, stream);
 }
 
-// Segments of a call: enough workgroups for two on every CU and again as many, so that requests of unequal length even
-// out; a segment is 256 rows at least, since one costs a state's round through memory. Sizes alone decide.
+// Segments of a call: as many as give every CU two workgroups, or with several requests four, so that requests of unequal
+// length even out; a segment is 256 rows at least, since one costs a state's round through memory. Sizes alone decide.
 struct Cut {
     int segs, seg_rows;
 };
 Cut cut(int heads, int batch, int max_rows) {
-    const ll groups = (ll)heads * batch;
-    ll segs = (1024 + groups - 1) / groups;
-    const ll most = ((ll)max_rows + 255) / 256;
+    const ll groups = (ll)heads * batch, most = ((ll)max_rows + 255) / 256;
+    ll segs = batch == 1 ? 512 / groups : (1024 + groups - 1) / groups;
     if (segs > most) segs = most;
-    if (groups >= 512 || segs < 1) segs = 1;
-    ll rows = ((ll)max_rows + segs - 1) / segs;
-    rows = (rows + C - 1) / C * C;
-    if (rows < C) rows = C;
-    if (segs == 1) return {1, (int)(rows > 0x7fffffff ? 0x7fffffe0 : rows)};
+    if (groups >= 512 || segs < 2) return {1, 0x7fffffc0};
+    const ll rows = (((ll)max_rows + segs - 1) / segs + 63) / 64 * 64;
     return {(int)(((ll)max_rows + rows - 1) / rows), (int)rows};
 }
 
@@ -633,7 +617,13 @@ int launch_prefill(const PrefillArgs<S>& a, int batch, hipStream_t stream) {
     return launched();
 }
 
-inline bool pair_rows(const void* p, ll stride) { return aligned(p, 4) && stride % 2 == 0; }
+template <typename S, int DK>
+int launch_prefill(const PrefillArgs<S>& a, int dv, bool fast, int batch, hipStream_t stream) {
+    if (dv == 64) return fast ? launch_prefill<S, DK, 2, true>(a, batch, stream) : launch_prefill<S, DK, 2, false>(a, batch, stream);
+    return fast ? launch_prefill<S, DK, 4, true>(a, batch, stream) : launch_prefill<S, DK, 4, false>(a, batch, stream);
+}
+
+inline bool whole_pieces(const void* p, ll stride) { return aligned(p, 16) && stride % 8 == 0; }
 
 template <typename S>
 int prefill(int heads, int qk_heads, int dk, int dv, int batch, int max_rows, const ChainArgs<S>& r, void* workspace,
@@ -646,16 +636,8 @@ int prefill(int heads, int qk_heads, int dk, int dv, int batch, int max_rows, co
     const PrefillArgs<S> a{heads, heads / qk_heads, max_rows, r.cu_rows, r.q, r.q_stride, r.k, r.k_stride, r.v, r.v_stride,
                            r.log_decay, r.scale, r.state_in, r.state_out, r.state_off, r.out, r.out_stride,
                            c.segs > 1 ? static_cast<float*>(workspace) : nullptr, c.segs, c.seg_rows};
-    const bool fast = pair_rows(r.q, r.q_stride) && pair_rows(r.k, r.k_stride) && pair_rows(r.v, r.v_stride) &&
-                      fast_rows(r.out, r.out_stride);
-    if (dk == 64) {
-        if (dv == 64)
-            return fast ? launch_prefill<S, 64, 2, true>(a, batch, stream) : launch_prefill<S, 64, 2, false>(a, batch, stream);
-        return fast ? launch_prefill<S, 64, 4, true>(a, batch, stream) : launch_prefill<S, 64, 4, false>(a, batch, stream);
-    }
-    if (dv == 64)
-        return fast ? launch_prefill<S, 128, 2, true>(a, batch, stream) : launch_prefill<S, 128, 2, false>(a, batch, stream);
-    return fast ? launch_prefill<S, 128, 4, true>(a, batch, stream) : launch_prefill<S, 128, 4, false>(a, batch, stream);
+    const bool fast = whole_pieces(r.q, r.q_stride) && whole_pieces(r.k, r.k_stride) && whole_pieces(r.v, r.v_stride);
+    return dk == 64 ? launch_prefill<S, 64>(a, dv, fast, batch, stream) : launch_prefill<S, 128>(a, dv, fast, batch, stream);
 }
 
 template <typename S>
