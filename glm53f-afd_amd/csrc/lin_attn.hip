@@ -320,20 +320,34 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
     const float g = a.log_decay[h];
     const ll row0 = (ll)first + begin, hk = h / a.group;
 
-    // Piece i of this thread: LDS slot t + T i of k's rows, then v's, then q's; row slot / pieces of a row. A row past the segment's
-    // last repeats it.
-    auto place_of = [&](int i) { return i < KN ? i * T * 8 : i < KN + VN ? C * DK + (i - KN) * T * 8 : C * (DK + DV) + (i - KN - VN) * T * 8; };
+    // Piece i of this thread: LDS slot t + T i of k's rows, then v's, then q's; row slot / pieces of a row. Whole chunks take it from
+    // a pointer that moves on; in the last one a row past the segment's end repeats the last.
+    auto is_v = [](int i) { return i >= KN && i < KN + VN; };
+    auto place_of = [&](int i) { return i < KN ? i * T * 8 : is_v(i) ? C * DK + (i - KN) * T * 8 : C * (DK + DV) + (i - KN - VN) * T * 8; };
+    auto slot_of = [&](int i) { return t + T * (i < KN ? i : is_v(i) ? i - KN : i - KN - VN); };
+    auto row_of = [&](int i) { return slot_of(i) / (is_v(i) ? VP : KP); };
+    auto stride_of = [&](int i) { return i < KN ? a.k_stride : is_v(i) ? a.v_stride : a.q_stride; };
+    const bf16_t* src[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int row = row_of(i), piece = (slot_of(i) % (is_v(i) ? VP : KP)) ^ (is_v(i) ? turn<VP>(row) : turn<KP>(row));
+        src[i] = (i < KN ? a.k + hk * DK : is_v(i) ? a.v + (ll)h * DV : a.q + hk * DK) + (row0 + row) * stride_of(i) + 8 * piece;
+    }
     u32x4_any held[FAST ? 1 : N];
     auto request = [&](int c, bf16_t* set) {
+        auto one = [&](int i, const bf16_t* from) {
+            if constexpr (FAST) to_lds(from, set + place_of(i) + wave * 512);
+            else held[i] = *reinterpret_cast<const u32x4_any*>(from);
+        };
+        if ((c + 1) * C <= n) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool is_v = i >= KN && i < KN + VN;
-            const int pieces = is_v ? VP : KP, slot = t + T * (i < KN ? i : is_v ? i - KN : i - KN - VN);
-            const int row = slot / pieces, piece = (slot % pieces) ^ (is_v ? turn<VP>(row) : turn<KP>(row));
-            const ll r = row0 + min(c * C + row, n - 1);
-            const bf16_t* src = i < KN ? a.k + r * a.k_stride + hk * DK : is_v ? a.v + r * a.v_stride + (ll)h * DV : a.q + r * a.q_stride + hk * DK;
-            if constexpr (FAST) to_lds(src + 8 * piece, set + place_of(i) + wave * 512);
-            else held[i] = *reinterpret_cast<const u32x4_any*>(src + 8 * piece);
+            for (int i = 0; i < N; ++i) {
+                one(i, src[i]);
+                src[i] += C * stride_of(i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) one(i, src[i] - max(c * C + row_of(i) - (n - 1), 0) * stride_of(i));
         }
     };
     auto place = [&](bf16_t* set) {               // the registers' pieces
@@ -494,7 +508,8 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
                 }
         }
         // the state behind the chunk
-        const float by = live == C ? whole : fade_of(g, live);
+        float by = whole;
+        if (live < C) by = fade_of(g, live);
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
             uint32_t kf[4];
