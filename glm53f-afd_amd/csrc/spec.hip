@@ -1,6 +1,6 @@
 // The two ends of a speculative round (gfx950): softmax rows of the LM head's logits, and the verification of drafted
 // tokens. Both are bound by the rows of the vocabulary that they read; a row is cut into segments, a workgroup each, so
-// that one row alone reaches many CUs, and a second launch joins the segments. A thread takes sixteen entries of its
+// that one row alone reaches many CUs, and a second launch joins the segments. A thread takes eight or sixteen entries of its
 // segment and requests them all before it looks at the first.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -12,8 +12,7 @@ namespace {
 
 constexpr int kInvalid = 1;                       // hipErrorInvalidValue
 constexpr int THREADS = 256, WAVES = THREADS / 64;
-constexpr int OWN = 16;                           // entries per thread
-constexpr int SEG = THREADS * OWN;                // entries of a row per workgroup
+constexpr int kMostVocab = 1 << 30;
 
 typedef long long ll;
 
@@ -92,10 +91,11 @@ __device__ __forceinline__ float wave_sum(float x) {
 // Groups of four (f32) or eight (bf16) entries go around the threads, so that a wave's access is contiguous.
 template <typename L> constexpr int kGroup = 16 / sizeof(L);
 
-template <typename L>
+// OWN: entries per thread, THREADS times as many per segment.
+template <typename L, int OWN>
 __global__ void __launch_bounds__(THREADS) probs_parts_kernel(int vocab, const L* logits, ll ldl, const float* temperature,
                                                               Part* parts) {
-    constexpr int G = kGroup<L>;
+    constexpr int G = kGroup<L>, SEG = THREADS * OWN;
     const int r = blockIdx.y, seg = blockIdx.x, t = threadIdx.x;
     const L* row = logits + r * ldl;
     float x[OWN / G][G];
@@ -131,10 +131,12 @@ __global__ void __launch_bounds__(THREADS) probs_parts_kernel(int vocab, const L
     if (t == 0) parts[(ll)r * gridDim.x + seg] = {top, (sums[0] + sums[1]) + (sums[2] + sums[3]), at, 0};
 }
 
-template <typename L>
+// The probabilities go past the caches (nontemporal), which keep the logits that the first pass has read: 384 rows of 151,936 f32
+// 114 us against 140.
+template <typename L, int OWN>
 __global__ void __launch_bounds__(THREADS) probs_write_kernel(int vocab, const L* logits, ll ldl, const float* temperature,
                                                               float* probs, ll ldp, const Part* parts) {
-    constexpr int G = kGroup<L>;
+    constexpr int G = kGroup<L>, SEG = THREADS * OWN;
     const int r = blockIdx.y, seg = blockIdx.x, segs = gridDim.x, t = threadIdx.x, lane = t & 63;
     const L* row = logits + r * ldl;
     float x[OWN / G][G];
@@ -167,7 +169,8 @@ __global__ void __launch_bounds__(THREADS) probs_write_kernel(int vocab, const L
             y[e] = rate != 0.0f ? share(x[j][e], top, rate) * by : i + e == at && top > kNone ? 1.0f : 0.0f;
         if (vocab - i >= G) {
 #pragma unroll
-            for (int e = 0; e < G; e += 4) *reinterpret_cast<f32x4*>(dst + i + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+            for (int e = 0; e < G; e += 4)
+                __builtin_nontemporal_store(f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]}, reinterpret_cast<f32x4*>(dst + i + e));
         } else {
 #pragma unroll
             for (int e = 0; e < G; ++e)
@@ -177,6 +180,10 @@ __global__ void __launch_bounds__(THREADS) probs_write_kernel(int vocab, const L
 }
 
 // ---------------------------------------------------------------------------------------------------- verification
+
+// Eight entries per thread: what a round waits for is the chain of loads (the windows, the tokens, their probabilities, the rows'
+// weights), so the rows are spread widely (one window 8.8 us, with sixteen 10.1; 64 windows 23.7 and 25.4).
+constexpr int OWN = 8, SEG = THREADS * OWN;
 
 __device__ __forceinline__ double weight(float p) { return p > 0.0f && p < __builtin_inff() ? (double)p : 0.0; }
 
@@ -399,15 +406,28 @@ __global__ void __launch_bounds__(THREADS) accept_pick_kernel(const Accept a, in
 }
 
 inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-inline ll segments(int vocab) { return ((ll)vocab + SEG - 1) / SEG; }
+inline ll segments(int vocab, int seg) { return ((ll)vocab + seg - 1) / seg; }
 
-template <typename L>
+// Entries per thread of the probabilities' passes: eight where sixteen would leave CUs without two workgroups (one row of 151,936 bf16
+// 7.8 us against 8.6), sixteen otherwise (384 rows f32 114 us against 130).
+inline int entries(int rows, int vocab) { return rows * segments(vocab, 16 * THREADS) < 512 ? 8 : 16; }
+
+// Both passes over a part of the rows at a time where the logits are more than the cache behind the L2 holds, so that the second
+// pass finds there what the first has read.
+constexpr ll kCached = 224LL << 20;
+
+template <typename L, int OWN>
 int32_t probs(int rows, int vocab, const void* logits, ll ldl, const float* temperature, float* out, ll ldp, Part* parts,
               hipStream_t stream) {
-    const dim3 grid((unsigned)segments(vocab), (unsigned)rows);
     const L* x = static_cast<const L*>(logits);
-    probs_parts_kernel<L><<<grid, THREADS, 0, stream>>>(vocab, x, ldl, temperature, parts);
-    probs_write_kernel<L><<<grid, THREADS, 0, stream>>>(vocab, x, ldl, temperature, out, ldp, parts);
+    const ll slabs = ((ll)rows * vocab * (ll)sizeof(L) + kCached - 1) / kCached;
+    const int most = (int)((rows + slabs - 1) / slabs);
+    for (int r = 0; r < rows; r += most) {
+        const dim3 grid((unsigned)segments(vocab, THREADS * OWN), (unsigned)(rows - r < most ? rows - r : most));
+        const float* t = temperature ? temperature + r : nullptr;
+        probs_parts_kernel<L, OWN><<<grid, THREADS, 0, stream>>>(vocab, x + r * ldl, ldl, t, parts);
+        probs_write_kernel<L, OWN><<<grid, THREADS, 0, stream>>>(vocab, x + r * ldl, ldl, t, out + r * ldp, ldp, parts);
+    }
     return (int32_t)hipGetLastError();
 }
 
@@ -415,28 +435,29 @@ int32_t probs(int rows, int vocab, const void* logits, ll ldl, const float* temp
 }  // namespace spec
 
 extern "C" int64_t glm53f_spec_probs_workspace_bytes(int32_t rows, int32_t vocab) {
-    if (rows < 0 || rows > 65535 || vocab < 1) return -1;
-    return rows * spec::segments(vocab) * (int64_t)sizeof(spec::Part);
+    if (rows < 0 || rows > 65535 || vocab < 1 || vocab > spec::kMostVocab) return -1;
+    return rows * spec::segments(vocab, spec::THREADS * spec::entries(rows, vocab)) * (int64_t)sizeof(spec::Part);
 }
 
 extern "C" int32_t glm53f_spec_probs(int32_t rows, int32_t vocab, const void* logits, int32_t logits_f32, int64_t ldl,
                                      const float* temperature, float* probs, int64_t ldp, void* workspace,
                                      int64_t workspace_bytes, ihipStream_t* stream) {
     using namespace spec;
-    if (rows < 0 || rows > 65535 || vocab < 1 || ldl < vocab || ldp < vocab) return kInvalid;
+    if (rows < 0 || rows > 65535 || vocab < 1 || vocab > kMostVocab || ldl < vocab || ldp < vocab) return kInvalid;
     if (rows == 0) return 0;
     if (!logits || !probs || !workspace || !aligned(logits, logits_f32 ? 4 : 2) || !aligned(probs, 4) ||
         !aligned(temperature, 4) || !aligned(workspace, 16) || workspace_bytes < glm53f_spec_probs_workspace_bytes(rows, vocab))
         return kInvalid;
     if (logits == probs && (!logits_f32 || ldl != ldp)) return kInvalid;
     Part* parts = static_cast<Part*>(workspace);
-    return logits_f32 ? spec::probs<float>(rows, vocab, logits, ldl, temperature, probs, ldp, parts, stream)
-                      : spec::probs<uint16_t>(rows, vocab, logits, ldl, temperature, probs, ldp, parts, stream);
+    auto* call = entries(rows, vocab) == 8 ? (logits_f32 ? &spec::probs<float, 8> : &spec::probs<uint16_t, 8>)
+                                           : (logits_f32 ? &spec::probs<float, 16> : &spec::probs<uint16_t, 16>);
+    return call(rows, vocab, logits, ldl, temperature, probs, ldp, parts, stream);
 }
 
 extern "C" int64_t glm53f_spec_accept_workspace_bytes(int32_t batch, int32_t vocab) {
-    if (batch < 0 || batch > 65535 || vocab < 1) return -1;
-    return batch * (spec::segments(vocab) * (int64_t)sizeof(double) + (int64_t)sizeof(int32_t));
+    if (batch < 0 || batch > 65535 || vocab < 1 || vocab > spec::kMostVocab) return -1;
+    return batch * (spec::segments(vocab, spec::SEG) * (int64_t)sizeof(double) + (int64_t)sizeof(int32_t));
 }
 
 extern "C" int32_t glm53f_spec_accept(int32_t batch, int32_t vocab, const int32_t* cu_rows, const int32_t* tokens,
@@ -444,13 +465,13 @@ extern "C" int32_t glm53f_spec_accept(int32_t batch, int32_t vocab, const int32_
                                       const float* uniform, int32_t* keep, int32_t* next, void* workspace,
                                       int64_t workspace_bytes, ihipStream_t* stream) {
     using namespace spec;
-    if (batch < 0 || batch > 65535 || vocab < 1 || p_stride < vocab || (draft && q_stride < vocab)) return kInvalid;
+    if (batch < 0 || batch > 65535 || vocab < 1 || vocab > kMostVocab || p_stride < vocab || (draft && q_stride < vocab)) return kInvalid;
     if (batch == 0) return 0;
     if (!cu_rows || !tokens || !target || !uniform || !keep || !next || !workspace || !aligned(cu_rows, 4) ||
         !aligned(tokens, 4) || !aligned(target, 4) || !aligned(draft, 4) || !aligned(uniform, 4) || !aligned(keep, 4) ||
         !aligned(next, 4) || !aligned(workspace, 16) || workspace_bytes < glm53f_spec_accept_workspace_bytes(batch, vocab))
         return kInvalid;
-    const int segs = (int)segments(vocab);
+    const int segs = (int)segments(vocab, SEG);
     double* parts = static_cast<double*>(workspace);
     int32_t* outcomes = reinterpret_cast<int32_t*>(parts + (ll)batch * segs);
     const Accept a{vocab, cu_rows, tokens, target, p_stride, draft, q_stride, uniform};

@@ -7,7 +7,8 @@
  * success, 1 (hipErrorInvalidValue) when the host rejects an argument, otherwise the launch error. Asynchronous on
  * `stream`, on the current device; nothing is allocated, freed or synchronized inside; device arrays are not read on the
  * host; may be captured into a graph. A workspace's contents do not matter before a call and mean nothing after it;
- * calls that may run at the same time need one each.
+ * calls that may run at the same time need one each. A call takes at most 65,535 rows or requests and a vocabulary of at most
+ * 2^30.
  */
 #ifndef GLM53F_SPEC_H
 #define GLM53F_SPEC_H

@@ -146,3 +146,10 @@ def test_workspaces_and_empty_calls():
     assert spec.glm53f_spec_probs_workspace_bytes(3, 151936) > 0 < spec.glm53f_spec_accept_workspace_bytes(3, 151936)
     assert probs_call(rows=0, x=None, p=None, ws=None) == 0 and accept_call(batch=0, cu=None, ws=None) == 0
     assert gemm_call(rows=0, x=None, o=None) == 0
+
+
+def test_a_vocabulary_past_its_bound_is_rejected():
+    big = (1 << 30) + 1
+    assert probs_call(vocab=big, ldl=big, ldp=big, wb=1 << 40) == 1 and accept_call(vocab=big, ps=big, qs=big, wb=1 << 40) == 1
+    assert spec.glm53f_spec_probs_workspace_bytes(1, big) == spec.glm53f_spec_accept_workspace_bytes(1, big) == -1
+    assert spec.glm53f_spec_probs_workspace_bytes(65536, 8) == spec.glm53f_spec_accept_workspace_bytes(65536, 8) == -1

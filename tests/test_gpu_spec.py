@@ -298,3 +298,23 @@ def test_a_round_from_logits_to_a_committed_kda_state():
         step(None)
         hs.sync()
         assert a[0] == keep.tolist() and a[1] == token.tolist() and torch.equal(a[2], probs) and torch.equal(a[3], pool), replay
+
+
+def test_probabilities_of_more_rows_than_the_caches_hold():
+    """The rows go in parts; each part's rows, the last one's too, come out as by themselves (a row's sums do not depend on
+    the rows beside it while the number of rows leaves the cut alone)."""
+    rows, vocab = 700, 90001
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(rows, vocab, generator=gen, device=DEV) * 3
+    t = torch.rand(rows, generator=gen, device=DEV) + 0.3
+    out = torch.zeros(rows, vocab, device=DEV)
+    need = ffi.glm53f_spec_probs_workspace_bytes(rows, vocab)
+    ws = torch.zeros(need, dtype=torch.uint8, device=DEV)
+    assert ffi.glm53f_spec_probs(rows, vocab, ptr(x), 1, vocab, ptr(t), ptr(out), vocab, ptr(ws), need, None) == 0
+    for at in (0, 333, 699):
+        want = torch.softmax(x[at].double() / t[at].double(), 0)
+        assert bool(((out[at].double() - want).abs() <= 2.0 ** -24 * (4 * 60 + 112) * want + 2.0 ** -126).all()), at
+    part = torch.zeros(100, vocab, device=DEV)
+    assert ffi.glm53f_spec_probs(100, vocab, ptr(x[600:]), 1, vocab, ptr(t[600:]), ptr(part), vocab, ptr(ws), need, None) == 0
+    hs.sync()
+    assert torch.equal(part, out[600:])
