@@ -436,7 +436,11 @@ int32_t probs(int rows, int vocab, const void* logits, ll ldl, const float* temp
 
 extern "C" int64_t glm53f_spec_probs_workspace_bytes(int32_t rows, int32_t vocab) {
     if (rows < 0 || rows > 65535 || vocab < 1 || vocab > spec::kMostVocab) return -1;
-    return rows * spec::segments(vocab, spec::THREADS * spec::entries(rows, vocab)) * (int64_t)sizeof(spec::Part);
+    // Fewer rows may be cut more finely: the most that any number up to `rows` needs, so that one workspace serves them all.
+    const int64_t whole = spec::segments(vocab, 16 * spec::THREADS), halves = spec::segments(vocab, 8 * spec::THREADS);
+    const int64_t few = 511 / whole < rows ? 511 / whole : rows;
+    const int64_t fine = few * halves, coarse = few < rows ? rows * whole : 0;
+    return (fine > coarse ? fine : coarse) * (int64_t)sizeof(spec::Part);
 }
 
 extern "C" int32_t glm53f_spec_probs(int32_t rows, int32_t vocab, const void* logits, int32_t logits_f32, int64_t ldl,

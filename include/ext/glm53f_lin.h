@@ -86,7 +86,9 @@ int32_t glm53f_lin_advance_batch_bf16state(int32_t heads, int32_t qk_heads, int3
 
 /**
  * Bytes of workspace that glm53f_lin_prefill_batch needs for these sizes: 0 where it needs none (short prompts, or
- * enough heads and requests to fill the GPU), -1 on arguments that it would reject.
+ * enough heads and requests to fill the GPU), -1 on arguments that it would reject. For exactly these sizes: fewer
+ * requests or rows may need more. Never more than 1,535 * key_dim * value_dim * 4, nor than
+ * heads * batch * ceil(max_rows / 256) * key_dim * value_dim * 4: the smaller of the two serves every call up to these sizes.
  */
 int64_t glm53f_lin_prefill_workspace_bytes(int32_t heads, int32_t key_dim, int32_t value_dim, int32_t batch,
     int32_t max_rows);

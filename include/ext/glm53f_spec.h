@@ -21,7 +21,7 @@ extern "C" {
 
 struct ihipStream_t;
 
-/** Bytes of workspace of glm53f_spec_probs for these sizes; -1 on arguments that it would reject. */
+/** Bytes of workspace of glm53f_spec_probs for these sizes, or fewer rows; -1 on arguments that it would reject. */
 int64_t glm53f_spec_probs_workspace_bytes(int32_t rows, int32_t vocab);
 
 /** probs[r][t] = softmax over t < vocab of logits[r][t] / temperature[r], for r < rows (0 succeeds without a launch).
@@ -37,7 +37,7 @@ int32_t glm53f_spec_probs(int32_t rows, int32_t vocab, const void* logits, int32
                           const float* temperature, float* probs, int64_t ldp, void* workspace,
                           int64_t workspace_bytes, struct ihipStream_t* stream);
 
-/** Bytes of workspace of glm53f_spec_accept for these sizes; -1 on arguments that it would reject. */
+/** Bytes of workspace of glm53f_spec_accept for these sizes, or fewer requests; -1 on arguments that it would reject. */
 int64_t glm53f_spec_accept_workspace_bytes(int32_t batch, int32_t vocab);
 
 /** The verification of a round's drafted tokens (speculative sampling: what is emitted is distributed as the target).
