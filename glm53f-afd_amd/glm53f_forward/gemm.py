@@ -1,7 +1,7 @@
 """The forward's BF16 weight GEMMs (reference: crates/glm53f-forward/src/gemm.rs:1-291): up to `gemv_max_rows` rows
 (8) run the hand-written GEMV of this library, bandwidth-bound and row-independent, so that a verify window of R rows
 gives the bits of R serial decode steps; more rows run the vendor GEMM (hipBLASLt through torch.matmul here, cuBLAS
-in the reference): BF16 inputs, f32 accumulation. The FP8 and MXFP8 paths of the reference's module are not part of
+in the reference): BF16 inputs, f32 accumulation. `fused` is the product with bias, activation and residual in one launch. The FP8 and MXFP8 paths of the reference's module are not part of
 the KDA layers' BF16 projections and are not built.
 """
 from dataclasses import dataclass
@@ -38,6 +38,21 @@ class Bf16Mat:
         if t.dim() == 2:
             return Bf16Mat(t.data_ptr(), t.shape[0], t.shape[1], t.shape[1])
         return Bf16Mat(t.data_ptr(), t.shape[1], t.shape[2], t.shape[2], t.shape[0], t.shape[1] * t.shape[2])
+
+
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh", "sigmoid")   # GLM53F_ACT_* of include/ext/glm53f_fwd_gemm.h
+
+
+@dataclass(frozen=True)
+class Epilogue:
+    """What follows a product in the same launch: out = residual + act(x . w + bias). Device addresses; 0: none. The
+    residual is of the outputs' type and may be `out` itself."""
+    bias: int = 0
+    b_gstride: int = 0
+    act: str = "none"
+    residual: int = 0
+    ldr: int = 0
+    r_gstride: int = 0
 
 
 @dataclass(frozen=True)
@@ -91,6 +106,19 @@ class Gemm:
                                              int(out_f32), ldo, o_gstride, stream)
         if rc != 0:
             raise GemmError("glm53f_fwd_gemm_bf16_skinny rejected its arguments" if rc == 1 else f"glm53f_fwd_gemm_bf16_skinny: hipError {rc}")
+
+    @staticmethod
+    def fused(x: int, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, epilogue: Epilogue, out: int, ldo: int, o_gstride: int,
+              out_f32: bool, stream: int = 0) -> None:
+        """The product with bias, activation and residual, for any rows (no counterpart in the reference, whose layers
+        launch elementwise kernels behind the GEMM)."""
+        if epilogue.act not in ACTIVATIONS:
+            raise GemmError(f"unknown activation {epilogue.act}")
+        rc = ffi.glm53f_fwd_gemm_bf16_fused(x, ldx, x_gstride, w.ptr, w.ld, w.gstride, w.groups, rows, w.n, w.k, epilogue.bias or None,
+                                            epilogue.b_gstride, ACTIVATIONS.index(epilogue.act), epilogue.residual or None,
+                                            epilogue.ldr, epilogue.r_gstride, out, int(out_f32), ldo, o_gstride, stream)
+        if rc != 0:
+            raise GemmError("glm53f_fwd_gemm_bf16_fused rejected its arguments" if rc == 1 else f"glm53f_fwd_gemm_bf16_fused: hipError {rc}")
 
     def gemv(self, x: int, ldx: int, x_gstride: int, w: Bf16Mat, rows: int, out: int, ldo: int, o_gstride: int,
              out_f32: bool, stream: int = 0) -> None:

@@ -3,7 +3,7 @@
 // new, bytes, gemv_ksplit, bf16, gemv, cublas) and of src/cublas.rs:98-245 (GemmDesc, Blas), with hipBLAS where the
 // reference binds cuBLAS. One dispatch more than the reference's: between the GEMV (up to 8 rows) and the vendor GEMM
 // sits this library's weight-streaming GEMM for 9 to 64 rows (glm53f_fwd_gemm_bf16_skinny); `skinny_max_rows = 0`
-// gives the reference's dispatch. The FP8 and MXFP8 paths of gemm.rs are not part of the KDA layers' BF16 projections
+// gives the reference's dispatch. And one product more: with its epilogue (Epilogue, Gemm::fused). The FP8 and MXFP8 paths of gemm.rs are not part of the KDA layers' BF16 projections
 // and are not mirrored. Header only; link with the kernel library, amdhip64 and hipblas.
 #ifndef GLM53F_FORWARD_HOST_GEMM_HPP
 #define GLM53F_FORWARD_HOST_GEMM_HPP
@@ -17,6 +17,7 @@
 #include <utility>
 
 #include "device.hpp"
+#include "ext/glm53f_fwd_gemm.h"
 #include "glm53f_fwd_gemv.h"
 
 namespace glm53f_forward {
@@ -39,6 +40,13 @@ struct GemmPolicy {
     /// GEMMs with more rows than that, up to this many (64 at most), run the library's GEMM for 9 to 64 rows where
     /// its shape rules allow; 0: never, everything above the GEMV goes to the vendor GEMM as in the reference.
     size_t skinny_max_rows = 64;
+};
+
+/// What follows a product in the same launch: out = residual + act(x . w + bias) (include/ext/glm53f_fwd_gemm.h).
+struct Epilogue {
+    const uint16_t* bias = nullptr; size_t b_gstride = 0;             // BF16 [groups][n]
+    int32_t act = GLM53F_ACT_NONE;
+    const void* residual = nullptr; size_t ldr = 0, r_gstride = 0;    // of the outputs' type; may be `out` itself
 };
 
 constexpr size_t kPartialFloats = size_t(1) << 20;   // split-K partial sums (gemm.rs:143)
@@ -215,6 +223,19 @@ class Gemm {
                                                     (int32_t)w.k, out, out_f32 ? 1 : 0, (int64_t)ldo, (int64_t)o_gstride,
                                                     stream.raw()),
                         "glm53f_fwd_gemm_bf16_skinny");
+    }
+
+    /// The product with bias, activation and residual, for any rows (no counterpart in the reference, whose layers launch
+    /// elementwise kernels behind the GEMM).
+    static Error fused(const uint16_t* x, size_t ldx, size_t x_gstride, const Bf16Mat& w, size_t rows, const Epilogue& e, void* out,
+                       size_t ldo, size_t o_gstride, bool out_f32, const Stream& stream) {
+        if (rows > (size_t)INT_MAX || w.n > (size_t)INT_MAX || w.k > (size_t)INT_MAX || w.groups > 65535)
+            return Error::invalid("glm53f_fwd_gemm_bf16_fused: sizes do not fit in 32 bits");
+        return launched(glm53f_fwd_gemm_bf16_fused(x, (int64_t)ldx, (int64_t)x_gstride, w.ptr, (int64_t)w.ld, (int64_t)w.gstride,
+                                                   (int32_t)w.groups, (int32_t)rows, (int32_t)w.n, (int32_t)w.k, e.bias,
+                                                   (int64_t)e.b_gstride, e.act, e.residual, (int64_t)e.ldr, (int64_t)e.r_gstride, out,
+                                                   out_f32 ? 1 : 0, (int64_t)ldo, (int64_t)o_gstride, stream.raw()),
+                        "glm53f_fwd_gemm_bf16_fused");
     }
 
     /// The vendor GEMM, whatever the policy, on the stream the engine was created on (gemm.rs:293-325).

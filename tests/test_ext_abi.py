@@ -153,3 +153,32 @@ def test_a_vocabulary_past_its_bound_is_rejected():
     assert probs_call(vocab=big, ldl=big, ldp=big, wb=1 << 40) == 1 and accept_call(vocab=big, ps=big, qs=big, wb=1 << 40) == 1
     assert spec.glm53f_spec_probs_workspace_bytes(1, big) == spec.glm53f_spec_accept_workspace_bytes(1, big) == -1
     assert spec.glm53f_spec_probs_workspace_bytes(65536, 8) == spec.glm53f_spec_accept_workspace_bytes(65536, 8) == -1
+
+
+@pytest.mark.parametrize("vocab", [1, 4096, 4097, 151936, 2_100_000])
+def test_a_workspace_serves_fewer_rows_too(vocab):
+    sizes = [spec.glm53f_spec_probs_workspace_bytes(r, vocab) for r in range(0, 700)]
+    assert sizes == sorted(sizes) and sizes[0] == 0
+    for rows, size in enumerate(sizes):
+        assert size >= rows * -(-vocab // 4096) * 16
+
+
+@pytest.mark.parametrize("heads,dk,dv", [(1, 64, 64), (16, 128, 128), (48, 64, 128), (300, 128, 64)])
+def test_the_documented_bound_of_the_chunked_forms_workspace(heads, dk, dv):
+    for batch in list(range(1, 70)) + [511, 512, 600]:
+        for rows in (0, 1, 256, 257, 512, 700, 4096, 8191, 100_000, 1 << 30):
+            need = lin.glm53f_lin_prefill_workspace_bytes(heads, dk, dv, batch, rows)
+            assert 0 <= need <= min(1535, heads * batch * -(-rows // 256)) * dk * dv * 4
+            if rows <= 256:
+                assert need == 0
+
+
+def test_the_gemms_python_wrapper():
+    from glm53f_forward import gemm
+    w = gemm.Bf16Mat(A, 32, 64, 64)
+    with pytest.raises(gemm.GemmError):
+        gemm.Gemm.fused(A, 64, 0, w, 4, gemm.Epilogue(act="swish"), A, 32, 0, False)
+    with pytest.raises(gemm.GemmError):
+        gemm.Gemm.fused(A, 63, 0, w, 4, gemm.Epilogue(act="silu"), A, 32, 0, False)
+    gemm.Gemm.fused(A, 64, 0, w, 0, gemm.Epilogue(act="silu"), A, 32, 0, False)       # no rows: no launch
+    assert gemm.ACTIVATIONS.index("gelu_tanh") == 4 and gemm.ACTIVATIONS.index("sigmoid") == 5
