@@ -295,6 +295,57 @@ __device__ __forceinline__ float* work_at(float* work, ll index) {
     return work + index * (32 * NW * DK) + (threadIdx.x >> 6) * (32 * DK) + (threadIdx.x & 63) * 4;
 }
 
+__device__ __forceinline__ bool finite(f32x4 a, f32x4 b) {
+    return ((a[0] + a[1]) + (a[2] + a[3]) + ((b[0] + b[1]) + (b[2] + b[3]))) * 0.0f == 0.0f;
+}
+
+// A segment's outputs once more, of one wave's values and row by row: where v has held an infinity or a NaN. The products of
+// a chunk cannot keep it from the rows before it, whose zero scores times it are NaN. Sixteen values at a time, four lanes each.
+template <typename S, int DK, int NW>
+__device__ void outputs_by_rows(const PrefillArgs<S>& a, const S* state, const float* start, ll row0, int n, int h, float g) {
+    constexpr int KEYS = DK / 4, DV = 32 * NW;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, key0 = (lane & 3) * KEYS;
+    const float fade = expf(g);
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+        const int r = 16 * half + (lane >> 2), col = 4 * (r >> 3) + (r & 3), x = r >> 2 & 1;   // value r of the wave's: tile x, column col
+        float s[KEYS];
+#pragma unroll
+        for (int i = 0; i < KEYS; i += 4) {
+            const int key = key0 + i, t = 2 * (key / 32) + (key >> 2 & 1), grp = key % 32 / 8;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (start) s[i + e] = start[wave * (32 * DK) + (2 * t + x) * 256 + (16 * grp + col) * 4 + e];
+                else if constexpr (sizeof(S) == 4) s[i + e] = state[(32 * wave + r) * DK + key + e];
+                else s[i + e] = kda::bf2f(state[(32 * wave + r) * DK + key + e]);
+            }
+        }
+        const bf16_t* k = a.k + row0 * a.k_stride + (h / a.group) * DK + key0;
+        const bf16_t* q = a.q + row0 * a.q_stride + (h / a.group) * DK + key0;
+        const bf16_t* v = a.v + row0 * a.v_stride + (ll)h * DV + 32 * wave + r;
+        bf16_t* out = a.out + row0 * a.out_stride + (ll)h * DV + 32 * wave + r;
+#pragma unroll 1
+        for (int t = 0; t < n; ++t, k += a.k_stride, q += a.q_stride, v += a.v_stride, out += a.out_stride) {
+            const float y = kda::bf2f(*v);
+            float o = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KEYS; i += 8) {
+                bf16_t ks[8], qs[8];
+                load_row<8>(k + i, ks);
+                load_row<8>(q + i, qs);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    s[i + e] = __builtin_fmaf(y, kda::bf2f(ks[e]), fade * s[i + e]);
+                    o = __builtin_fmaf(s[i + e], kda::bf2f(qs[e]) * a.scale, o);
+                }
+            }
+            o += kda::lane_xor16<2>(o);
+            o += kda::lane_xor16<1>(o);
+            if ((lane & 3) == 0) *out = kda::f2bf(o);
+        }
+    }
+}
+
 // SUMS: what the segment adds to a state, into the workspace; otherwise its outputs, and behind a request's last row
 // the state. FAST: the rows of q, k and v are 16-byte aligned and go straight to LDS; otherwise through registers.
 template <typename S, int DK, int NW, bool FAST, bool SUMS>
@@ -402,6 +453,7 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
     const int at_v0 = C * DK + tr0 * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr0)), at_v1 = C * DK + tr1 * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr1));
 
     int set = 0;
+    bool odd = false;                             // a chunk's first row shows any infinity or NaN of its v
     for (int c = 0; c * C < n; ++c, set = SET - set) {
         const int live = min(n - c * C, C);
         bf16_t* now = lds + set;
@@ -482,6 +534,7 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
                     store_row<8>(a.out + (row0 + c * C + 16 * i + col) * a.out_stride + (ll)h * DV + 32 * wave + 8 * grp, y);
                 }
             }
+            odd |= !finite(o[0][0], o[1][0]);
             if (a.state_out == nullptr && last && (c + 1) * C >= n) break;   // nobody reads the state behind the last rows
         }
         // v decayed to the chunk's end, in terms
@@ -531,7 +584,13 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
         for (int m = 0; m < KT; ++m)
 #pragma unroll
             for (int x = 0; x < 2; ++x) *reinterpret_cast<f32x4*>(w + (2 * m + x) * 256) = s[m][x];
-    } else if (last && a.state_out) {
+    } else {
+        if (__any(odd)) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the outputs so far are written
+            const float* start = a.work ? a.work + (((ll)b * a.heads + h) * a.segs + seg) * (DV * DK) : nullptr;
+            outputs_by_rows<S, DK, NW>(a, a.state_in + state_at, start, row0, n, h, g);
+        }
+        if (!last || !a.state_out) return;
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll

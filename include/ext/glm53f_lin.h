@@ -28,7 +28,8 @@
  * the call stores it. Products of bf16 values are exact; sums are f32. Outputs are rounded to bf16 once.
  * `glm53f_lin_chain_batch` and `glm53f_lin_advance_batch` give a state the same bits for the same rows, and with f32
  * states a window of R rows has the bits of R calls with one row. The chunked form agrees within f32 rounding of the
- * terms, not bit for bit.
+ * terms, not bit for bit. A value of q, k or v that is not finite does not reach earlier rows' outputs or
+ * other requests; where it reaches, outputs and states are infinite or NaN, not always the one that the formula gives.
  */
 #ifndef GLM53F_LIN_H
 #define GLM53F_LIN_H
@@ -48,7 +49,8 @@ struct ihipStream_t;
  *            A request without rows keeps its state (it is copied where state_out is another buffer). Rows that belong
  *            to no request are neither read nor written.
  * state_off  int64 [batch]: request b's state is state_in + state_off[b], written to state_out + state_off[b].
- *            Regions of different requests must not overlap.
+ *            Regions of different requests must not overlap, but may be the same where state_out is NULL (several windows
+ *            behind one state).
  * state_out  the states behind the last row: equal to state_in (in place), disjoint from it, or NULL (not written: a
  *            verify window).
  */

@@ -414,3 +414,66 @@ def test_bits_do_not_depend_on_the_requests_beside():
                                           None) == 0
     hs.sync()
     assert torch.equal(hs_bits(alone), hs_bits(pool)) and torch.equal(p.out_rows(), want)
+
+
+@pytest.mark.parametrize("form", ["prefill", "chain"])
+@pytest.mark.parametrize("shape", [(4, 2, 128, 128), (3, 1, 64, 64), (2, 2, 128, 64), (2, 1, 64, 128)])
+@pytest.mark.parametrize("what", ["v", "k", "q"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_a_value_that_is_not_finite_reaches_no_earlier_row(form, shape, what, value):
+    """Planted in one row of a prompt of several chunks (and segments), and in the last rows of a short one: the rows before
+    it, the other heads and requests are right as without it; the rows that the recurrence carries it to are not finite."""
+    lens, shift = [700, 5, 40], 0 if value > 0 else 1
+    clean, bad = (Problem(shape, lens, False, seed=91, shift=shift) for _ in range(2))
+    heads, qk, dk, dv = shape
+    group, col = heads // qk, {"q": 0, "k": qk * dk, "v": 2 * qk * dk}[what]
+    head, lane = (heads - 1, dv - 3) if what == "v" else (qk - 1, dk - 5)
+    rows = [(0, 333), (0, 699), (1, 3), (2, 0)] if what == "q" else [(0, 333), (1, 3), (2, 39)]
+    first = [0, 700, 705]
+    plant = bad.rows.cpu()
+    at = lambda r: shift + (bad.ahead + r) * bad.stride + col + head * (dv if what == "v" else dk) + lane  # noqa: E731
+    for b, t in rows:
+        plant[at(first[b] + t)] = value
+    bad.rows.copy_(plant)
+    for p in (clean, bad):
+        pool = p.pool.to(DEV)
+        need = ffi.glm53f_lin_prefill_workspace_bytes(*(shape[0], dk, dv), 3, 700)
+        ws = torch.zeros(max(need, 16), dtype=torch.uint8, device=DEV)
+        assert (p.call(form, pool, pool, workspace=ws) if form == "prefill" else p.call(form, pool, pool)) == 0
+    hs.sync()
+    want, got = (p.out_rows().reshape(745, heads, dv) for p in (clean, bad))
+    touched = torch.zeros(745, heads, dv, dtype=torch.bool)
+    for b, t in rows:
+        r, end = first[b] + t, first[b] + lens[b]
+        if what == "v":
+            touched[r:end, head, lane] = True
+        elif what == "k":
+            touched[r:end, head * group:(head + 1) * group] = True
+        else:
+            touched[r, head * group:(head + 1) * group] = True
+    assert bool(torch.isfinite(want).all())
+    for b, n in enumerate(lens):
+        here, free = slice(first[b], first[b] + n), ~touched[first[b]:first[b] + n]
+        o, _, ao, _ = clean.oracle(b)
+        tol = 2.0 ** -8 * o.abs() + ((n + dk + 16) * 2.0 ** -24 + (2.0 ** -16 if form == "prefill" else 0)) * ao + 1e-30
+        within(got[here][free], o[free], tol[free], f"what it cannot reach of request {b}")
+    assert not bool(torch.isfinite(got[touched]).any()), "a row that it reaches is finite"
+
+
+@pytest.mark.parametrize("form", ["prefill", "chain"])
+def test_windows_of_one_state(form):
+    """Several windows behind the same state (drafts of one prompt): nothing is written, so the regions may be the same."""
+    p = Problem((4, 2, 128, 128), [5, 5, 16], False, seed=97)
+    p.off[1:] = p.off[0]
+    pool = p.pool.to(DEV)
+    assert p.call(form, pool, None) == 0
+    hs.sync()
+    slot = p.pool[p.order[0]]
+    state = slot.reshape(4, 128, 128)
+    at = 0
+    for m in p.lens:
+        o, _, ao, _ = lo.attention(p.q[at:at + m], p.k[at:at + m], p.v[at:at + m], p.g, p.scale, state)
+        got = p.out_rows().reshape(-1, 4, 128)[at:at + m].double()
+        within(got, o, 2.0 ** -8 * o.abs() + (2.0 ** -15 + (m + 144) * 2.0 ** -24) * ao, form)
+        at += m
+    assert torch.equal(pool[p.order[0]].cpu(), slot)
