@@ -68,7 +68,8 @@ __device__ __forceinline__ bool before(float x, int i, float y, int j) { return 
 __device__ __forceinline__ float rate_of(const float* temperature, int r) {
     const float t = temperature ? temperature[r] : 1.0f;
     if (!(t > 0.0f)) return 0.0f;                 // the greatest logit alone
-    return fminf(1.0f / t, 3.0e38f);              // finite, so that 0 times it is 0
+    // finite, so that 0 times it is 0; above 0, since 0 stands for the case above (an infinite temperature: all alike)
+    return fmaxf(fminf(1.0f / t, 3.0e38f), 1.0e-45f);
 }
 
 // exp((x - top) * rate), 0 for -inf (also where nothing else is there and top is -inf).

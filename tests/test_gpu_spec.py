@@ -318,3 +318,18 @@ def test_probabilities_of_more_rows_than_the_caches_hold():
     assert ffi.glm53f_spec_probs(100, vocab, ptr(x[600:]), 1, vocab, ptr(t[600:]), ptr(part), vocab, ptr(ws), need, None) == 0
     hs.sync()
     assert torch.equal(part, out[600:])
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_an_infinite_temperature_is_uniform(kind):
+    gen = torch.Generator().manual_seed(8)
+    x = (torch.randn(3, 4999, generator=gen) * 30).to(kind)
+    x[1, 7:90] = -math.inf
+    x[2] = -math.inf
+    got = spec_probs(x, torch.full((3,), math.inf)).double()
+    left = (x > -math.inf).double()
+    want = left / left.sum(1, keepdim=True).clamp(min=1)
+    assert bool(((got - want).abs() <= 2.0 ** -24 * 112 * want).all())
+    got = spec_probs(x, torch.tensor([3e38, 1e-45, 1.0]))
+    assert bool(((got[0].double() - 1 / 4999).abs() <= 2.0 ** -24 * 112).all())
+    assert int(got[1].argmax()) == int(x[1].float().argmax()) and abs(float(got[1].sum()) - 1) < 1e-6 and bool((got[2] == 0).all())
