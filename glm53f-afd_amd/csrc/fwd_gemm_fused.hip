@@ -18,6 +18,7 @@ using fwd_stream::u32x4_any;
 
 constexpr int kInvalid = 1;                       // hipErrorInvalidValue
 constexpr int kCus = 256;
+constexpr int kMostSize = 1 << 30;                // of rows, n and k: tiles' counts and ends stay below 2^31
 
 struct Args {
     const uint16_t* x;
@@ -378,7 +379,8 @@ extern "C" int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, in
                                               const void* residual, int64_t ldr, int64_t r_gstride, void* out,
                                               int32_t out_f32, int64_t ldo, int64_t o_gstride, ihipStream_t* stream) {
     using namespace fwd_fused;
-    if (groups < 1 || groups > 65535 || rows < 0 || n < 1 || k < 1 || act < GLM53F_ACT_NONE || act > GLM53F_ACT_SIGMOID)
+    if (groups < 1 || groups > 65535 || rows < 0 || n < 1 || k < 1 || rows > kMostSize || n > kMostSize || k > kMostSize ||
+        act < GLM53F_ACT_NONE || act > GLM53F_ACT_SIGMOID)
         return kInvalid;
     if (ldx < k || ldw < k || ldo < n || x_gstride < 0 || w_gstride < 0 || o_gstride < 0 ||
         (bias && b_gstride < 0) || (residual && (ldr < n || r_gstride < 0)))

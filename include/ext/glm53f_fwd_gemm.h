@@ -30,11 +30,13 @@ struct ihipStream_t;
  *  for g < groups, m < rows, o < n: x row m at x + g*x_gstride + m*ldx, w row o at w + g*w_gstride + o*ldw, bias at
  *  bias + g*b_gstride (bf16, NULL: none), residual at residual + g*r_gstride + m*ldr (of the outputs' type, NULL: none),
  *  out at out + g*o_gstride + m*ldo (bf16, or f32 when out_f32 != 0).
- *  Any rows, n, k >= 1 (rows == 0 succeeds without a launch), ldx, ldw >= k, ldo, ldr >= n, group strides >= 0; pointers
+ *  Any rows, n, k from 1 to 2^30 (rows == 0 succeeds without a launch), groups from 1 to 65,535, ldx, ldw >= k, ldo,
+ *  ldr >= n, group strides >= 0; pointers
  *  aligned to their elements. 16-byte aligned x and w with strides and k that are multiples of 8 are read fastest.
  *  residual may be out itself with the same strides (the residual stream updated in place); otherwise out overlaps no
  *  input. Outputs of different groups must not overlap.
- *  Numerics: exact bf16 products, f32 sums over k, the epilogue in f32, one rounding to the outputs' type. */
+ *  Numerics: exact bf16 products, f32 sums over k, the epilogue in f32 (an activation of y within 2^-20 (1 + |y|)), one
+ *  rounding to the outputs' type. */
 int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, int64_t x_gstride, const uint16_t* w, int64_t ldw,
                                    int64_t w_gstride, int32_t groups, int32_t rows, int32_t n, int32_t k,
                                    const uint16_t* bias, int64_t b_gstride, int32_t act, const void* residual,

@@ -182,3 +182,8 @@ def test_the_gemms_python_wrapper():
         gemm.Gemm.fused(A, 63, 0, w, 4, gemm.Epilogue(act="silu"), A, 32, 0, False)
     gemm.Gemm.fused(A, 64, 0, w, 0, gemm.Epilogue(act="silu"), A, 32, 0, False)       # no rows: no launch
     assert gemm.ACTIVATIONS.index("gelu_tanh") == 4 and gemm.ACTIVATIONS.index("sigmoid") == 5
+
+
+@pytest.mark.parametrize("bad", [dict(rows=(1 << 30) + 1), dict(n=(1 << 30) + 1, ldo=1 << 31, ldr=1 << 31), dict(k=(1 << 30) + 1, ldx=1 << 31, ldw=1 << 31)])
+def test_a_product_past_its_bounds_is_rejected(bad):
+    assert gemm_call(**bad) == 1
