@@ -18,6 +18,7 @@ struct Epilogue {
     void* out;
     int out_f32;
     long long ldo, o_gs;
+    int early;                                    // the residual may be requested in 16-byte pieces
 };
 
 __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }

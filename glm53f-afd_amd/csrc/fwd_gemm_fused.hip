@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
     constexpr int SETS = FAST ? STAGES : 2, SET = (BM + BN) * BK;
     constexpr int PASSES = KW * BM * BN * 4 > (128 << 10) ? 2 : 1, ROWS = BM / PASSES;   // the outputs take the tiles' place, in passes
     constexpr int CELLS = SETS * SET > KW * ROWS * BN * 2 ? SETS * SET : KW * ROWS * BN * 2;
-    __shared__ __align__(16) uint16_t lds[CELLS];
+    constexpr int SPARE = FAST ? T * 8 : 0;               // where the residual's early requests go
+    __shared__ __align__(16) uint16_t lds[CELLS + SPARE];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = blockIdx.z;
     // Consecutive workgroups go to the eight XCDs in turn: give each XCD a run of tiles, and order the tiles in bands of
     // eight rows of tiles, column by column, so that the tiles that run at a time on an XCD are a block of both operands
@@ -143,6 +144,18 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
                 }
             }
     };
+    // The residual's tile is asked for during the last steps, into a corner that nobody reads: the epilogue then finds it in the
+    // caches (2048 rows 8192 -> 4096 134 -> 129 us, 124 without a residual; 1024 -> 4096 41 -> 37; 4096 rows 4096 -> 8192
+    // 313 -> 295).
+    const int res = a.e.early ? (a.e.out_f32 ? BM * BN / 4 / T : BM * BN / 8 / T) : 0, res_from = max(steps - res - 4, 0);
+    auto early = [&](int step) {
+        const int i = step - res_from, per = a.e.out_f32 ? 4 : 8, slot = i * T + t;
+        if (i < 0 || i >= res) return;
+        const long long row = min(m0 + slot / (BN / per), (long long)a.rows - 1);
+        const int o = min(n0 + slot % (BN / per) * per, (a.n - per) & -per);
+        const long long cell = g * a.e.r_gs + row * a.e.ldr + o;
+        to_lds(static_cast<const uint16_t*>(a.e.residual) + (a.e.out_f32 ? 2 * cell : cell), lds + CELLS + wave * 512);
+    };
     if constexpr (FAST && BK == 32) {
         // The operands of the next step are read while the current one's products run.
         bf16x8 f[2][MT + NT];
@@ -173,6 +186,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
             const int before = set == 0 ? STAGES - 1 : set - 1;
             set = set == STAGES - 1 ? 0 : set + 1;
             read(set, then);
+            early(s);
             request(s + STAGES - 1, before);
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
@@ -191,6 +205,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
         for (int s = 0; s < STAGES - 1; ++s) request(s, s);
         int set = 0;
         for (int s = 0; s < steps; ++s) {
+            early(s);
             // this wave's part of the set is there once all but the newer steps' requests have come back; behind the
             // barrier everybody's is, and nobody reads the set before it any more, which the newest request fills
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(P * (STAGES - 2)) : "memory");
@@ -391,12 +406,14 @@ extern "C" int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, in
         !aligned(residual, cell))
         return kInvalid;
     if (residual == out && (ldr != ldo || (groups > 1 && r_gstride != o_gstride))) return kInvalid;
-    const Args a{x, ldx, x_gstride, w, ldw, w_gstride, groups, rows, n, k,
-                 Epilogue{bias, b_gstride, act, residual, ldr, r_gstride, out, out_f32, ldo, o_gstride}, stream};
+    Args a{x, ldx, x_gstride, w, ldw, w_gstride, groups, rows, n, k,
+           Epilogue{bias, b_gstride, act, residual, ldr, r_gstride, out, out_f32, ldo, o_gstride, 0}, stream};
     if (k < 8) {
         short_kernel<<<dim3((unsigned)((n + 255LL) / 256), (unsigned)(rows < 1024 ? rows : 1024), (unsigned)groups), 256, 0, stream>>>(a);
         return (int32_t)hipGetLastError();
     }
+    const int per = out_f32 ? 4 : 8;
+    a.e.early = residual && n >= per && aligned(residual, 16) && ldr % per == 0 && r_gstride % per == 0;
     const bool fast = aligned(x, 16) && aligned(w, 16) && ldx % 8 == 0 && ldw % 8 == 0 && x_gstride % 8 == 0 &&
                       w_gstride % 8 == 0;
     // Up to 64 rows the weights stream past the rows once; with up to 256 too where a workgroup per sixteen outputs and 64 rows is at

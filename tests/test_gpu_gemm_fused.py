@@ -195,3 +195,25 @@ def test_a_captured_product_replays_like_eager_products():
 
 def test_no_rows_is_no_launch():
     assert ffi.glm53f_fwd_gemm_bf16_fused(None, 8, 0, None, 8, 0, 1, 0, 8, 8, None, 0, 0, None, 0, 0, None, 0, 8, 0, None) == 0
+
+
+@pytest.mark.parametrize("rows,n,k", [(65, 203, 128), (300, 203, 192), (513, 1001, 64), (1025, 4099, 256), (2100, 8190, 64), (300, 7, 128), (70, 3, 128)])
+@pytest.mark.parametrize("f32_out", [False, True])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_residual_rows_whose_stride_is_longer_than_they_are(rows, n, k, f32_out, in_place):
+    """Aligned rows of x, w and the residual, n of no multiple: what the residual's tile is asked for early ends at the rows'
+    ends. The columns behind are NaN in the residual and stay what they are in the outputs."""
+    gen = torch.Generator().manual_seed(rows + n)
+    kind, ld = (torch.float32 if f32_out else torch.bfloat16), (n + 15) // 8 * 8
+    x, w = torch.randn(rows, k, generator=gen).bfloat16(), (torch.randn(n, k, generator=gen) * k ** -0.5).bfloat16()
+    res = torch.full((rows, ld), math.nan, dtype=kind)
+    res[:, :n] = torch.randn(rows, n, generator=gen).to(kind)
+    d_x, d_w, d_r = x.to(DEV), w.to(DEV), res.to(DEV)
+    d_o = d_r if in_place else torch.full((rows, ld), math.nan, dtype=kind, device=DEV)
+    assert ffi.glm53f_fwd_gemm_bf16_fused(ptr(d_x), k, 0, ptr(d_w), k, 0, 1, rows, n, k, None, 0, 0, ptr(d_r), ld, 0, ptr(d_o), int(f32_out),
+                                          ld, 0, None) == 0
+    hs.sync()
+    got = d_o.cpu().double()
+    want, a = lo.gemm(x, w, None, 0, res[:, :n])
+    tol = 1.13 * (k + 1) * 2.0 ** -24 * a + 2.0 ** -24 * want.abs() + 1e-30 + (0 if f32_out else 2.0 ** -8 * want.abs())
+    assert bool(((got[:, :n] - want).abs() <= tol).all()) and bool(got[:, n:].isnan().all())
