@@ -52,9 +52,14 @@ __device__ __forceinline__ void to_lds(const uint16_t* src, uint16_t* lds) {
 // BM rows x BN outputs per workgroup of WM x WN waves, k in steps of BK, a ring of STAGES sets of LDS tiles: the steps ahead
 // are requested before the current one's products, STAGES - 1 of them. A tile row is BK / 8 pieces of 16 bytes in LDS,
 // swizzled by the row so that the sixteen rows of an operand's read fall on all banks. With 16-byte aligned rows and k a
-// multiple of BK (FAST) the tiles go straight to LDS, the swizzle in the lanes' addresses; otherwise through registers, a
-// piece that crosses the row's end shifted and filled with zeros. Rows past the last repeat it and are not stored.
-template <int BM, int BN, int WM, int WN, int KW, int BK, int STAGES, bool FAST>
+// multiple of 8 (FAST) the tiles go straight to LDS, the swizzle in the lanes' addresses, and where k is no multiple of BK
+// (TAIL) the pieces behind the rows' ends come from a piece of zeros (2048 rows 8200 -> 4096 136 us, through registers 163; 200
+// rows 4104 -> 4096 23 and 31; 1024 rows, whose stride parts every row's run over two lines, 59 and 57); otherwise through
+// registers, a piece that crosses the row's end shifted and filled with zeros. Rows past the last repeat it and are not
+// stored.
+__device__ const u32x4 kZeros[1] = {};
+
+template <int BM, int BN, int WM, int WN, int KW, int BK, int STAGES, bool FAST, bool TAIL>
 __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
     constexpr int T = 64 * WM * WN * KW, MT = BM / WM / 16, NT = BN / WN / 16, PR = BK / 8;
     constexpr int XP = BM * PR / T, WP = BN * PR / T, P = XP + WP;   // pieces per thread of a step
@@ -94,8 +99,10 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
     auto slot_of = [&](int i, int set) { return lds + set * SET + (i < XP ? i * T * 8 : BM * BK + (i - XP) * T * 8); };
     auto request_piece = [&](int i, int step, int set) {   // (behind the last step it is requested again: the waits count requests)
         step = min(step, steps - 1);
+        const uint16_t* from = src[i] + step * BK + col[i];
+        if constexpr (TAIL) from = step * BK + col[i] < a.k ? from : reinterpret_cast<const uint16_t*>(kZeros);
         if constexpr (FAST)
-            to_lds(src[i] + step * BK + col[i], slot_of(i, set) + wave * 512);
+            to_lds(from, slot_of(i, set) + wave * 512);
         else
             held[set][i] = *reinterpret_cast<const u32x4_any*>(src[i] + min(step * BK + col[i], a.k - 8));
     };
@@ -331,11 +338,11 @@ int32_t stream_rows(const Args& a) {
     return stream_split<4, 4, ANY>(a);
 }
 
-template <int BM, int BN, int WM, int WN, int KW, int BK, int STAGES, bool FAST>
+template <int BM, int BN, int WM, int WN, int KW, int BK, int STAGES, bool FAST, bool TAIL = false>
 int32_t tiles(const Args& a) {
     const long long count = (long long)((a.rows + (long long)BM - 1) / BM) * ((a.n + (long long)BN - 1) / BN);
     if (count > 0x7fffffff) return kInvalid;
-    tile_kernel<BM, BN, WM, WN, KW, BK, STAGES, FAST>
+    tile_kernel<BM, BN, WM, WN, KW, BK, STAGES, FAST, TAIL>
         <<<dim3((unsigned)count, 1, (unsigned)a.groups), 64 * WM * WN * KW, 0, a.stream>>>(a);
     return (int32_t)hipGetLastError();
 }
@@ -345,7 +352,7 @@ int32_t tiles(const Args& a) {
 // but in whole rounds of 256: the shape whose rounds take least time is launched. Measured with one round, 8192 k:
 // 128 rows -> 4096 29 us with 64 x 32 tiles, 42 with 64 x 64; 400 rows 44 us with 128 x 64, 61 with 128 x 128, 101 with
 // 64 x 32 (four rounds); 1024 rows 71 us with 128 x 128, 110 with 128 x 256; 2048 rows 124 us with 128 x 256, 136 with
-// 128 x 128; 4096 rows 224 us with 256 x 256, 240 with 128 x 256. Rows at any address take 1.7 times as long, all shapes alike.
+// 128 x 128; 4096 rows 224 us with 256 x 256, 240 with 128 x 256. Rows at any address take 1.3 to 1.8 times as long.
 enum Shape { k64x32, k64x64, k128x64, k128x128, k128x256, k256x256 };
 Shape shape_of(const Args& a, bool fast) {
     constexpr struct { int bm, bn; double us; } table[] = {{64, 32, 0.20}, {64, 64, 0.31}, {128, 64, 0.33},
@@ -361,19 +368,23 @@ Shape shape_of(const Args& a, bool fast) {
     return (Shape)best;
 }
 
+template <bool TAIL>
+int32_t aligned_tiles(const Args& a, Shape shape) {
+    switch (shape) {
+        case k64x32: return tiles<64, 32, 1, 1, 4, 128, 4, true, TAIL>(a);
+        case k64x64: return tiles<64, 64, 1, 1, 4, 128, 4, true, TAIL>(a);
+        case k128x64: return tiles<128, 64, 2, 1, 4, 128, 3, true, TAIL>(a);
+        case k128x128: return tiles<128, 128, 2, 2, 2, 64, 4, true, TAIL>(a);
+        case k128x256: return tiles<128, 256, 2, 4, 1, 64, 3, true, TAIL>(a);
+        default: return tiles<256, 256, 2, 4, 1, 32, 4, true, TAIL>(a);
+    }
+}
+
 int32_t tiled(const Args& a, bool fast) {
     const Shape shape = shape_of(a, fast);
-    // k a multiple of 128 for the narrow tiles, whose four waves share a step's k, of 64 for the others
-    if (fast && a.k % 128 == 0) {
-        if (shape == k64x32) return tiles<64, 32, 1, 1, 4, 128, 4, true>(a);
-        if (shape == k64x64) return tiles<64, 64, 1, 1, 4, 128, 4, true>(a);
-        if (shape == k128x64) return tiles<128, 64, 2, 1, 4, 128, 3, true>(a);
-    }
-    if (fast && a.k % 64 == 0) {
-        if (shape == k128x128) return tiles<128, 128, 2, 2, 2, 64, 4, true>(a);
-        if (shape == k128x256) return tiles<128, 256, 2, 4, 1, 64, 3, true>(a);
-        if (shape == k256x256) return tiles<256, 256, 2, 4, 1, 32, 4, true>(a);
-    }
+    // whole steps are of 128 k with the narrow tiles, whose four waves share a step's k, of 64 with the others
+    const bool narrow = shape <= k128x64;
+    if (fast) return a.k % (narrow ? 128 : 64) == 0 ? aligned_tiles<false>(a, shape) : aligned_tiles<true>(a, shape);
     switch (shape) {
         case k64x32: return tiles<64, 32, 1, 1, 4, 128, 3, false>(a);
         case k64x64: return tiles<64, 64, 2, 2, 1, 64, 3, false>(a);
@@ -421,5 +432,5 @@ extern "C" int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, in
     const long long thin = (long long)((n + 15LL) / 16) * ((rows + 63LL) / 64) * groups;
     if (rows <= 64 || (rows <= 256 && thin <= kCus))
         return fast && n % 16 == 0 && k % 128 == 0 ? stream_rows<false>(a) : stream_rows<true>(a);
-    return tiled(a, fast);
+    return tiled(a, fast && k % 8 == 0);
 }

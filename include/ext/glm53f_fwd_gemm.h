@@ -31,8 +31,8 @@ struct ihipStream_t;
  *  bias + g*b_gstride (bf16, NULL: none), residual at residual + g*r_gstride + m*ldr (of the outputs' type, NULL: none),
  *  out at out + g*o_gstride + m*ldo (bf16, or f32 when out_f32 != 0).
  *  Any rows, n, k from 1 to 2^30 (rows == 0 succeeds without a launch), groups from 1 to 65,535, ldx, ldw >= k, ldo,
- *  ldr >= n, group strides >= 0; pointers
- *  aligned to their elements. 16-byte aligned x and w with strides and k that are multiples of 8 are read fastest.
+ *  ldr >= n, group strides >= 0; pointers aligned to their elements. 16-byte aligned x and w with strides and k that are
+ *  multiples of 8 are read fastest, of 128 best.
  *  residual may be out itself with the same strides (the residual stream updated in place); otherwise out overlaps no
  *  input. Outputs of different groups must not overlap.
  *  Numerics: exact bf16 products, f32 sums over k, the epilogue in f32 (an activation of y within 2^-20 (1 + |y|)), one

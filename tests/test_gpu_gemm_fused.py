@@ -217,3 +217,14 @@ def test_residual_rows_whose_stride_is_longer_than_they_are(rows, n, k, f32_out,
     want, a = lo.gemm(x, w, None, 0, res[:, :n])
     tol = 1.13 * (k + 1) * 2.0 ** -24 * a + 2.0 ** -24 * want.abs() + 1e-30 + (0 if f32_out else 2.0 ** -8 * want.abs())
     assert bool(((got[:, :n] - want).abs() <= tol).all()) and bool(got[:, n:].isnan().all())
+
+
+@pytest.mark.parametrize("rows,n,k", [(100, 2000, 8), (200, 4096, 264), (300, 4096, 72), (400, 2500, 1000), (513, 4096, 4104), (1025, 4096, 200),
+                                      (2049, 4096, 328), (4096, 4096, 72), (130, 77, 136)])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_aligned_rows_whose_k_is_no_whole_step(rows, n, k, groups):
+    """Every tile's shape with k a multiple of 8 and no more; NaN in the eight columns behind k, which no product may reach."""
+    if groups == 2 and rows > 600:
+        rows = rows // 8 + 1
+    run(groups, rows, n, k, "none", f32_out=True, pad=8, seed=k)
+    run(groups, rows, n, k, "silu", residual=False, seed=k + 1)
