@@ -1,5 +1,5 @@
-// The weight-streaming BF16 product for up to 64 rows a workgroup (gfx950): the projections of a decode or verify step with more rows than the
-// GEMV takes. Like the GEMV it is bound by the weight stream - every weight byte is read from HBM once with 128-bit
+// The weight-streaming BF16 product for up to 64 rows a workgroup (gfx950): the projections of a decode or verify step with
+// more rows than the GEMV takes. Like the GEMV it is bound by the weight stream - every weight byte is read from HBM once with 128-bit
 // nontemporal loads - but the arithmetic runs on the matrix cores: with sixteen rows a weight piece of 1 KiB is one
 // v_mfma_f32_16x16x32_bf16, so the vector units, which bound the GEMV from five rows up, do nothing here.
 //

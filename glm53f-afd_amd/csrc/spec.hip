@@ -182,6 +182,8 @@ __global__ void __launch_bounds__(THREADS) probs_write_kernel(int vocab, const L
 
 // ---------------------------------------------------------------------------------------------------- verification
 
+// Two launches: sums of segments and every request's outcome, then one workgroup per request that finds the token. 64 windows of up
+// to nine rows over 151,936 entries: 18.6 and 5.3 us (78 MB: 4.2 TB/s in the first), one window 3.9 and 4.7 (launches and chains).
 // Eight entries per thread: what a round waits for is the chain of loads (the windows, the tokens, their probabilities, the rows'
 // weights), so the rows are spread widely (one window 8.8 us, with sixteen 10.1; 64 windows 23.7 and 25.4).
 constexpr int OWN = 8, SEG = THREADS * OWN;
