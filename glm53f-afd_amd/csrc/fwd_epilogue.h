@@ -31,7 +31,7 @@ __device__ __forceinline__ float gated(float y, float z) {
 
 // y Phi(y), with erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2), t = 1 / (1 + 0.3275911 x) for x >= 0 (Abramowitz and Stegun,
 // Handbook of Mathematical Functions, 7.1.26: off by at most 1.5e-7); the far left keeps the factor e^(-x^2). A sixth of the
-// instructions of the library's erfc: 333 rows 1001 -> 1999 with GELU and an f32 residual 19.5 -> 15.2 us.
+// instructions of the library's erfc: 333 rows 1001 -> 1999 take 4 us less.
 __device__ __forceinline__ float gelu(float y) {
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(y), 1.0f));
     float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);

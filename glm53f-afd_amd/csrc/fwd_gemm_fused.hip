@@ -321,7 +321,9 @@ template <int NT, int TMAX, bool ANY>
 int32_t stream_split(const Args& a) {
     const long long tiles = (long long)((a.n + 15) / 16) * a.groups;
     if (tiles <= kCus && (ANY ? a.k >= 1024 : a.k % 1024 == 0)) {
-        if (!ANY && a.k % 2048 == 0 && (NT == 1 || tiles * NT <= kCus)) return stream<256, 1, 1, 8, ANY>(a);
+        // (sixteen rows a workgroup where they still are at most one per CU: 192 rows 2048 -> 1024 10.8 us otherwise, 7.7 so)
+        const long long row_tiles = a.rows <= 64 ? NT : (a.rows + 15) / 16;
+        if (!ANY && a.k % 2048 == 0 && (NT == 1 || tiles * row_tiles <= kCus)) return stream<256, 1, 1, 8, ANY>(a);
         return stream<128, NT, 1, 8, ANY>(a);
     }
     if (ANY ? a.k >= 512 : a.k % 512 == 0) {
@@ -349,20 +351,24 @@ int32_t tiles(const Args& a) {
 
 // The tile of a product of more than 64 rows. Each shape runs a workgroup per CU, and a step of 64 k takes it about the
 // time of the table, larger tiles less per output (fewer bytes through the CU's load path per product, which bounds them)
-// but in whole rounds of 256: the shape whose rounds take least time is launched. Measured with one round, 8192 k:
-// 128 rows -> 4096 29 us with 64 x 32 tiles, 42 with 64 x 64; 400 rows 44 us with 128 x 64, 61 with 128 x 128, 101 with
-// 64 x 32 (four rounds); 1024 rows 71 us with 128 x 128, 110 with 128 x 256; 2048 rows 124 us with 128 x 256, 136 with
-// 128 x 128; 4096 rows 224 us with 256 x 256, 240 with 128 x 256. Rows at any address take 1.3 to 1.8 times as long.
+// but in whole rounds of 256: the shape whose rounds take least time is launched. Measured 8192 -> 4096, us:
+//   rows            128   256   512  1024  2048  4096        at any address  128   256   512  1024  2048
+//   64 x 32          28    53   106   197   355   707                         45    75   138   239   445
+//   64 x 64          36    40    73   130   236   469                         56    59    97   166   311
+//   128 x 64         50    52    53    93   178   349                         96    92    90   152   256
+//   128 x 128        73    72    73    75   146   286                        131   124   119   113   199
+//   128 x 256       114   113   112   112   126   251                        209   199   193   183   172
+//   256 x 256       198   220   215   206   202   239
 enum Shape { k64x32, k64x64, k128x64, k128x128, k128x256, k256x256 };
 Shape shape_of(const Args& a, bool fast) {
-    constexpr struct { int bm, bn; double us; } table[] = {{64, 32, 0.20}, {64, 64, 0.31}, {128, 64, 0.33},
-                                                           {128, 128, 0.53}, {128, 256, 0.93}, {256, 256, 1.70}};
+    constexpr struct { int bm, bn; double aligned, any; } table[] = {{64, 32, 0.20, 0.33},   {64, 64, 0.29, 0.43},   {128, 64, 0.39, 0.67},
+                                                                     {128, 128, 0.56, 0.85}, {128, 256, 0.96, 1.31}, {256, 256, 1.85, 0.0}};
     int best = 0;
     double least = 1e300;
     for (int i = 0; i < (fast ? 6 : 5); ++i) {
         const double count = (double)((a.rows + (long long)table[i].bm - 1) / table[i].bm) *
                              (double)((a.n + (long long)table[i].bn - 1) / table[i].bn) * a.groups;
-        const double time = (double)(long long)((count + kCus - 1) / kCus) * table[i].us;
+        const double time = (double)(long long)((count + kCus - 1) / kCus) * (fast ? table[i].aligned : table[i].any);
         if (time < least) least = time, best = i;
     }
     return (Shape)best;
@@ -371,8 +377,8 @@ Shape shape_of(const Args& a, bool fast) {
 template <bool TAIL>
 int32_t aligned_tiles(const Args& a, Shape shape) {
     switch (shape) {
-        case k64x32: return tiles<64, 32, 1, 1, 4, 128, 4, true, TAIL>(a);
-        case k64x64: return tiles<64, 64, 1, 1, 4, 128, 4, true, TAIL>(a);
+        case k64x32: return tiles<64, 32, 2, 2, 2, 128, 4, true, TAIL>(a);
+        case k64x64: return tiles<64, 64, 2, 2, 2, 128, 4, true, TAIL>(a);
         case k128x64: return tiles<128, 64, 2, 1, 4, 128, 3, true, TAIL>(a);
         case k128x128: return tiles<128, 128, 2, 2, 2, 64, 4, true, TAIL>(a);
         case k128x256: return tiles<128, 256, 2, 4, 1, 64, 3, true, TAIL>(a);
@@ -386,10 +392,10 @@ int32_t tiled(const Args& a, bool fast) {
     const bool narrow = shape <= k128x64;
     if (fast) return a.k % (narrow ? 128 : 64) == 0 ? aligned_tiles<false>(a, shape) : aligned_tiles<true>(a, shape);
     switch (shape) {
-        case k64x32: return tiles<64, 32, 1, 1, 4, 128, 3, false>(a);
-        case k64x64: return tiles<64, 64, 2, 2, 1, 64, 3, false>(a);
-        case k128x64: return tiles<128, 64, 2, 1, 4, 128, 3, false>(a);
-        case k128x128: return tiles<128, 128, 2, 2, 2, 64, 3, false>(a);
+        case k64x32: return tiles<64, 32, 2, 1, 4, 128, 2, false>(a);
+        case k64x64: return tiles<64, 64, 2, 2, 2, 128, 2, false>(a);
+        case k128x64: return tiles<128, 64, 2, 2, 2, 64, 3, false>(a);
+        case k128x128: return tiles<128, 128, 2, 2, 2, 64, 2, false>(a);
         default: return tiles<128, 256, 2, 4, 1, 64, 3, false>(a);
     }
 }
@@ -428,7 +434,8 @@ extern "C" int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, in
     const bool fast = aligned(x, 16) && aligned(w, 16) && ldx % 8 == 0 && ldw % 8 == 0 && x_gstride % 8 == 0 &&
                       w_gstride % 8 == 0;
     // Up to 64 rows the weights stream past the rows once; with up to 256 too where a workgroup per sixteen outputs and 64 rows is at
-    // most one per CU (200 rows 4096 -> 512: 10 us against 15 with 64 x 32 tiles, which have as few).
+    // most one per CU (200 rows 4096 -> 512: 10.9 us against 13.1 with tiles; 128 rows 8192 -> 2048 20.6 and 25.3; 128 rows
+    // 512 -> 1024 4.8 and 4.9).
     const long long thin = (long long)((n + 15LL) / 16) * ((rows + 63LL) / 64) * groups;
     if (rows <= 64 || (rows <= 256 && thin <= kCus))
         return fast && n % 16 == 0 && k % 128 == 0 ? stream_rows<false>(a) : stream_rows<true>(a);
