@@ -67,7 +67,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
     static_assert(XP * T == BM * PR && WP * T == BN * PR, "whole pieces");
     constexpr int SETS = FAST ? STAGES : 2, SET = (BM + BN) * BK;
     constexpr int PASSES = KW * BM * BN * 4 > (128 << 10) ? 2 : 1, ROWS = BM / PASSES;   // the outputs take the tiles' place, in passes
-    constexpr int CELLS = SETS * SET > KW * ROWS * BN * 2 ? SETS * SET : KW * ROWS * BN * 2;
+    constexpr bool DIRECT = KW == 1 && MT * NT <= 16;                // a wave's outputs stored as they lie
+    constexpr int CELLS = DIRECT || SETS * SET > KW * ROWS * BN * 2 ? SETS * SET : KW * ROWS * BN * 2;
     constexpr int SPARE = FAST ? T * 8 : 0;               // where the residual's early requests go
     __shared__ __align__(16) uint16_t lds[CELLS + SPARE];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), g = blockIdx.z;
@@ -239,8 +240,29 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
             }
         }
     }
-    // acc[i][j][e]: row 16 i + lane % 16, output 16 j + 4 (lane / 16) + e of the wave's part. Through LDS (pieces of four
-    // outputs, swizzled like the tiles), so that a wave stores whole runs of a row and the epilogue is written once.
+    // acc[i][j][e]: row 16 i + lane % 16, output 16 j + 4 (lane / 16) + e of the wave's part. Where a wave has them whole and
+    // the registers hold what is added to a row of tiles beside them, they are stored from there (2048 rows 2048 -> 4096 39.3 us,
+    // through LDS 41.9; tiles of 256 x 256 spill).
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const long long m = m0 + wm + 16 * i + r16;
+            fwd_epilogue::Added added[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int o = n0 + wn + 16 * j + 4 * q;
+                if (m < a.rows && o < a.n) added[j] = fwd_epilogue::request(a.e, g, m, o, a.n);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int o = n0 + wn + 16 * j + 4 * q;
+                if (m < a.rows && o < a.n) fwd_epilogue::finish(a.e, added[j], g, m, o, a.n, acc[i][j]);
+            }
+        }
+        return;
+    }
+    // Otherwise through LDS (pieces of four outputs, swizzled like the tiles), where the waves' parts of k meet and a wave stores
+    // whole runs of a row.
     float* whole = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int pass = 0; pass < PASSES; ++pass) {
