@@ -35,7 +35,8 @@ __device__ __forceinline__ void load_row(const bf16_t* p, bf16_t (&e)[N]) {
     }
 }
 
-template <int N>
+// PAST: past the caches.
+template <int N, bool PAST = false>
 __device__ __forceinline__ void store_row(bf16_t* p, const float (&x)[N]) {
     if constexpr (N == 1) {
         p[0] = kda::f2bf(x[0]);
@@ -47,7 +48,8 @@ __device__ __forceinline__ void store_row(bf16_t* p, const float (&x)[N]) {
             vec w;
 #pragma unroll
             for (int c = 0; c < V / 2; ++c) w[c] = kda::f2bf2(x[i + 2 * c], x[i + 2 * c + 1]);
-            *reinterpret_cast<vec*>(p + i) = w;
+            if constexpr (PAST) __builtin_nontemporal_store(w, reinterpret_cast<vec*>(p + i));
+            else *reinterpret_cast<vec*>(p + i) = w;
         }
     }
 }
@@ -184,8 +186,8 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // all segments are computed from there at once. k and v are then read twice, the second time from the caches as far as
 // they hold them.
 //
-// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 203 us (under
-// the profiler, cold caches: what the segments add 70, 3.8 TB/s; the starts 13; the outputs 156, 3.4 TB/s). The card's copy
+// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 200 us (under
+// the profiler, cold caches: what the segments add 63, 4.3 TB/s; the starts 12; the outputs 140, 3.8 TB/s). The card's copy
 // rate is 5.1; what is left is the vector work (the state's terms and decay, the terms of v: half of the instruction
 // slots) that two waves a SIMD do not quite hide. The window of 48 requests of up to sixteen rows (bf16 states, nothing written) 34 us, 3 TB/s of states.
 
@@ -215,6 +217,7 @@ struct PrefillArgs {
     ll out_stride;
     float* work;                                  // [batch][heads][segs] states in the waves' order, NULL: one segment
     int segs, seg_rows;                           // seg_rows: a multiple of C
+    int past;                                     // the outputs go past the caches
 };
 
 // e^{g n}; 1 for n = 0 also where nothing is remembered (g = -inf).
@@ -355,8 +358,15 @@ __device__ void outputs_by_rows(const PrefillArgs<S>& a, const S* state, const f
 
 // SUMS: what the segment adds to a state, into the workspace; otherwise its outputs, and behind a request's last row
 // the state. FAST: the rows of q, k and v are 16-byte aligned and go straight to LDS; otherwise through registers.
+//
+// Waves per SIMD: three where the rows go straight to LDS, for the sums two and no more, though the registers would let
+// five in: a CU then takes another segment when one of its own ends, which evens out unequal lengths (nine ragged prompts 95 us,
+// with three 97, with five 105).
+constexpr int least_waves(bool fast, int nw, bool sums) { return fast && nw == 4 && !sums ? 3 : 2; }
+constexpr int most_waves(bool fast, int nw, bool sums) { return fast && nw == 4 ? (sums ? 2 : 3) : 8; }
 template <typename S, int DK, int NW, bool FAST, bool SUMS>
-__global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kernel(const PrefillArgs<S> a) {
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(least_waves(FAST, NW, SUMS), most_waves(FAST, NW, SUMS))))
+segment_kernel(const PrefillArgs<S> a) {
     constexpr int T = 64 * NW, KT = DK / 16, DV = 32 * NW, TERMS = 3;
     constexpr int KP = DK / 8, VP = DV / 8;                          // pieces of a row
     constexpr int QN = SUMS ? 0 : C * KP / T, KN = C * KP / T, VN = C * VP / T, N = QN + KN + VN;   // pieces per thread and chunk
@@ -379,7 +389,8 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
     const ll row0 = (ll)first + begin, hk = h / a.group;
 
     // Piece i of this thread: LDS slot t + T i of k's rows, then v's, then q's; row slot / pieces of a row. Whole chunks take it from
-    // a pointer that moves on; in the last one a row past the segment's end repeats the last.
+    // a pointer that moves on; in the last one a row past the segment's end repeats the last. The sums, whose segments are whole
+    // chunks, go from the last chunk to the first: what is read last is read first afterwards.
     auto is_v = [](int i) { return i >= KN && i < KN + VN; };
     auto place_of = [&](int i) { return i < KN ? i * T * 8 : is_v(i) ? C * DK + (i - KN) * T * 8 : C * (DK + DV) + (i - KN - VN) * T * 8; };
     auto slot_of = [&](int i) { return t + T * (i < KN ? i : is_v(i) ? i - KN : i - KN - VN); };
@@ -389,7 +400,7 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int row = row_of(i), piece = (slot_of(i) % (is_v(i) ? VP : KP)) ^ (is_v(i) ? turn<VP>(row) : turn<KP>(row));
-        src[i] = (i < KN ? a.k + hk * DK : is_v(i) ? a.v + (ll)h * DV : a.q + hk * DK) + (row0 + row) * stride_of(i) + 8 * piece;
+        src[i] = (i < KN ? a.k + hk * DK : is_v(i) ? a.v + (ll)h * DV : a.q + hk * DK) + (row0 + (SUMS ? n - C : 0) + row) * stride_of(i) + 8 * piece;
     }
     u32x4_any held[FAST ? 1 : N];
     auto request = [&](int c, bf16_t* set) {
@@ -397,11 +408,11 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
             if constexpr (FAST) to_lds(from, set + place_of(i) + wave * 512);
             else held[i] = *reinterpret_cast<const u32x4_any*>(from);
         };
-        if ((c + 1) * C <= n) {
+        if (SUMS || (c + 1) * C <= n) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 one(i, src[i]);
-                src[i] += C * stride_of(i);
+                src[i] += (SUMS ? -C : C) * stride_of(i);
             }
         } else {
 #pragma unroll
@@ -461,8 +472,8 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
 
     int set = 0;
     bool odd = false;                             // a chunk's first row shows any infinity or NaN of its v
-    for (int c = 0; c * C < n; ++c, set = SET - set) {
-        const int live = min(n - c * C, C);
+    for (int c = 0; c * C < n; ++c, set = SET - set) {               // SUMS: chunk n / C - 1 - c
+        const int live = SUMS ? C : min(n - c * C, C);
         bf16_t* now = lds + set;
         const bf16_t* qs = now + C * (DK + DV);
         // this thread's part of the chunk is there; behind the barrier everybody's is, and the other set is free
@@ -538,18 +549,20 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
                 }
                 if (16 * i + col < live) {
                     const float y[8] = {o[0][i][0], o[0][i][1], o[0][i][2], o[0][i][3], o[1][i][0], o[1][i][1], o[1][i][2], o[1][i][3]};
-                    store_row<8>(a.out + (row0 + c * C + 16 * i + col) * a.out_stride + (ll)h * DV + 32 * wave + 8 * grp, y);
+                    bf16_t* at = a.out + (row0 + c * C + 16 * i + col) * a.out_stride + (ll)h * DV + 32 * wave + 8 * grp;
+                    if (a.past) store_row<8, true>(at, y);
+                    else store_row<8>(at, y);
                 }
             }
             odd |= !finite(o[0][0], o[1][0]);
             if (a.state_out == nullptr && last && (c + 1) * C >= n) break;   // nobody reads the state behind the last rows
         }
-        // v decayed to the chunk's end, in terms
+        // v decayed to the chunk's end (SUMS: to the segment's, so that the sums need no decay), in terms
         uint32_t vd[TERMS][2][4];
         {
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = in_tail[e];
+            for (int e = 0; e < 8; ++e) f[e] = SUMS ? in_tail[e] * fade_of(g, c * C) : in_tail[e];
             if (live < C) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] = fade_of(g, max(live - 1 - (8 * grp + e), 0));
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(64 * NW, FAST && NW == 4 ? 3 : 2) segment_kern
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[m][x][e] *= by;
+                for (int e = 0; e < 4; ++e) s[m][x][e] *= SUMS ? 1.0f : by;
 #pragma unroll
                 for (int i = 0; i < TERMS; ++i) s[m][x] = product(operand(kf), operand(vd[i][x]), s[m][x]);
             }
@@ -714,9 +727,12 @@ int prefill(int heads, int qk_heads, int dk, int dv, int batch, int max_rows, co
     if (c.segs > 1 && (!workspace || !aligned(workspace, 16) ||
                        workspace_bytes < glm53f_lin_prefill_workspace_bytes(heads, dk, dv, batch, max_rows)))
         return kInvalid;
+    // Segments read k and v twice. Where they are about as large as the cache behind the L2 the outputs, written meanwhile, go
+    // past it (k and v of 268 MB: 204 us with them in, 198 past; of 100 MB 95 and 100).
+    const bool past = c.segs > 1 && (ll)batch * max_rows * ((ll)heads * dv + (ll)qk_heads * dk) * (ll)sizeof(bf16_t) > 192LL << 20;
     const PrefillArgs<S> a{heads, heads / qk_heads, max_rows, r.cu_rows, r.q, r.q_stride, r.k, r.k_stride, r.v, r.v_stride,
                            r.log_decay, r.scale, r.state_in, r.state_out, r.state_off, r.out, r.out_stride,
-                           c.segs > 1 ? static_cast<float*>(workspace) : nullptr, c.segs, c.seg_rows};
+                           c.segs > 1 ? static_cast<float*>(workspace) : nullptr, c.segs, c.seg_rows, past ? 1 : 0};
     const bool fast = whole_pieces(r.q, r.q_stride) && whole_pieces(r.k, r.k_stride) && whole_pieces(r.v, r.v_stride);
     return dk == 64 ? launch_prefill<S, 64>(a, dv, fast, batch, stream) : launch_prefill<S, 128>(a, dv, fast, batch, stream);
 }
