@@ -186,10 +186,10 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // all segments are computed from there at once. k and v are then read twice, the second time from the caches as far as
 // they hold them.
 //
-// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 200 us (under
-// the profiler, cold caches: what the segments add 63, 4.3 TB/s; the starts 12; the outputs 140, 3.8 TB/s). The card's copy
-// rate is 5.1; what is left is the vector work (the state's terms and decay, the terms of v: half of the instruction
-// slots) that two waves a SIMD do not quite hide. The window of 48 requests of up to sixteen rows (bf16 states, nothing written) 34 us, 3 TB/s of states.
+// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 200 us (under the profiler, cold
+// caches: what the segments add 63, the starts 12, the outputs 140). With k and v twice and eight segments' states
+// written and read twice that moves 940 MB, 184 us at the card's copy rate; a tenth fewer vector instructions (remainders
+// by dot products) changed nothing. The window of 48 requests of up to sixteen rows (bf16 states, nothing written) 34 us, 3 TB/s of states.
 
 constexpr int C = 32;                             // rows per chunk: one product's depth
 
