@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 200 us (under the profiler, cold
 // caches: what the segments add 63, the starts 12, the outputs 140). With k and v twice and eight segments' states
 // written and read twice that moves 940 MB, 184 us at the card's copy rate; a tenth fewer vector instructions (remainders
-// by dot products) changed nothing. The window of 48 requests of up to sixteen rows (bf16 states, nothing written) 34 us, 3 TB/s of states.
+// by dot products) changed nothing. The windows of 48 requests of up to sixteen rows (bf16 states, only read) 22.7 us, 4.4
+// TB/s of states.
 
 constexpr int C = 32;                             // rows per chunk: one product's depth
 
@@ -362,18 +363,25 @@ __device__ void outputs_by_rows(const PrefillArgs<S>& a, const S* state, const f
 // Waves per SIMD: three where the rows go straight to LDS, for the sums two and no more, though the registers would let
 // five in: a CU then takes another segment when one of its own ends, which evens out unequal lengths (nine ragged prompts 95 us,
 // with three 97, with five 105).
-constexpr int least_waves(bool fast, int nw, bool sums) { return fast && nw == 4 && !sums ? 3 : 2; }
-constexpr int most_waves(bool fast, int nw, bool sums) { return fast && nw == 4 ? (sums ? 2 : 3) : 8; }
-template <typename S, int DK, int NW, bool FAST, bool SUMS>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(least_waves(FAST, NW, SUMS), most_waves(FAST, NW, SUMS))))
+//
+// ONCE: windows of one chunk whose states are only read. Nothing is double then, no state is kept behind the product that reads
+// it, and a bf16 state is its operand as it lies in memory, so that more workgroups share a CU's loads (48 windows of up to
+// sixteen rows of 64 heads, bf16 states: 22.7 us against 34).
+constexpr int least_waves(bool fast, int nw, bool sums, bool once) { return once ? (nw == 4 ? 4 : 2) : fast && nw == 4 && !sums ? 3 : 2; }
+constexpr int most_waves(bool fast, int nw, bool sums, bool once) { return fast && nw == 4 && !once ? (sums ? 2 : 3) : 8; }
+template <typename S, int DK, int NW, bool FAST, bool SUMS, bool ONCE>
+__global__ void __launch_bounds__(64 * NW)
+__attribute__((amdgpu_waves_per_eu(least_waves(FAST, NW, SUMS, ONCE), most_waves(FAST, NW, SUMS, ONCE))))
 segment_kernel(const PrefillArgs<S> a) {
     constexpr int T = 64 * NW, KT = DK / 16, DV = 32 * NW, TERMS = 3;
     constexpr int KP = DK / 8, VP = DV / 8;                          // pieces of a row
     constexpr int QN = SUMS ? 0 : C * KP / T, KN = C * KP / T, VN = C * VP / T, N = QN + KN + VN;   // pieces per thread and chunk
     static_assert(C * KP % T == 0 && C * VP % T == 0, "whole pieces");
     constexpr int SET = (SUMS ? 1 : 2) * C * DK + C * DV;            // a chunk's rows in LDS: k, v, q
-    __shared__ __align__(16) bf16_t lds[2 * SET + (SUMS ? 0 : 2 * C * C)];
-    bf16_t* ph = lds + 2 * SET;                                      // the scores' terms [row][column]
+    constexpr int SETS = ONCE ? 1 : 2;
+    constexpr bool RAW = ONCE && sizeof(S) == 2;                     // the state's operands as they lie in memory
+    __shared__ __align__(16) bf16_t lds[SETS * SET + (SUMS ? 0 : 2 * C * C)];
+    bf16_t* ph = lds + SETS * SET;                                    // the scores' terms [row][column]
     bf16_t* pl = ph + C * C;
     const int h = blockIdx.x % a.heads, seg = blockIdx.x / a.heads, b = blockIdx.y;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), col = lane & 15, grp = lane >> 4;
@@ -428,7 +436,14 @@ segment_kernel(const PrefillArgs<S> a) {
     if (n > 0) request(0, lds);
 
     f32x4 s[KT][2];
-    if constexpr (SUMS) {
+    kda::u32x4_t raw[KT / 2][2];
+    if constexpr (RAW) {
+#pragma unroll
+        for (int u = 0; u < KT / 2; ++u)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                raw[u][x] = *reinterpret_cast<const kda::u32x4_t*>(a.state_in + state_at + value_of(x, wave, col) * DK + 32 * u + 8 * grp);
+    } else if constexpr (SUMS) {
 #pragma unroll
         for (int m = 0; m < KT; ++m) s[m][0] = s[m][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     } else if (a.work) {
@@ -524,6 +539,11 @@ segment_kernel(const PrefillArgs<S> a) {
                 const bf16x8 q0 = operand(qs + (at_row ^ (32 * u))), q1 = operand(qs + (at_row16 ^ (32 * u)));
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
+                    if constexpr (RAW) {
+                        o[x][0] = product(__builtin_bit_cast(bf16x8, raw[u][x]), q0, o[x][0]);
+                        o[x][1] = product(__builtin_bit_cast(bf16x8, raw[u][x]), q1, o[x][1]);
+                        continue;
+                    }
                     float z[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[e] = s[2 * u][x][e], z[4 + e] = s[2 * u + 1][x][e];
@@ -555,7 +575,7 @@ segment_kernel(const PrefillArgs<S> a) {
                 }
             }
             odd |= !finite(o[0][0], o[1][0]);
-            if (a.state_out == nullptr && last && (c + 1) * C >= n) break;   // nobody reads the state behind the last rows
+            if (ONCE || (a.state_out == nullptr && last && (c + 1) * C >= n)) break;   // nobody reads the state behind the last rows
         }
         // v decayed to the chunk's end (SUMS: to the segment's, so that the sums need no decay), in terms
         uint32_t vd[TERMS][2][4];
@@ -610,7 +630,7 @@ segment_kernel(const PrefillArgs<S> a) {
             const float* start = a.work ? a.work + (((ll)b * a.heads + h) * a.segs + seg) * (DV * DK) : nullptr;
             outputs_by_rows<S, DK, NW>(a, a.state_in + state_at, start, row0, n, h, g);
         }
-        if (!last || !a.state_out) return;
+        if (ONCE || !last || !a.state_out) return;
 #pragma unroll
         for (int m = 0; m < KT; ++m)
 #pragma unroll
@@ -704,10 +724,13 @@ template <typename S, int DK, int NW, bool FAST>
 int launch_prefill(const PrefillArgs<S>& a, int batch, hipStream_t stream) {
     const dim3 grid((unsigned)((ll)a.heads * a.segs), (unsigned)batch);
     if (a.segs > 1) {
-        segment_kernel<S, DK, NW, FAST, true><<<grid, 64 * NW, 0, stream>>>(a);
+        segment_kernel<S, DK, NW, FAST, true, false><<<grid, 64 * NW, 0, stream>>>(a);
         starts_kernel<S, DK, NW><<<dim3((unsigned)a.heads, (unsigned)batch, 2 * (DK / 16)), 64 * NW, 0, stream>>>(a);
     }
-    segment_kernel<S, DK, NW, FAST, false><<<grid, 64 * NW, 0, stream>>>(a);
+    if (a.segs == 1 && a.state_out == nullptr && a.most <= C)
+        segment_kernel<S, DK, NW, FAST, false, true><<<grid, 64 * NW, 0, stream>>>(a);
+    else
+        segment_kernel<S, DK, NW, FAST, false, false><<<grid, 64 * NW, 0, stream>>>(a);
     return launched();
 }
 

@@ -477,3 +477,40 @@ def test_windows_of_one_state(form):
         within(got, o, 2.0 ** -8 * o.abs() + (2.0 ** -15 + (m + 144) * 2.0 ** -24) * ao, form)
         at += m
     assert torch.equal(pool[p.order[0]].cpu(), slot)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("bf16_state", [False, True])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 8), (3, 1)])
+@pytest.mark.parametrize("lens", [[1, 16, 0, 5, 32], [7, 33, 2]])
+def test_windows_that_only_read_their_states(shape, bf16_state, pad, shift, lens):
+    """Windows of one chunk (no state is written) in every head size, and one that is a row longer."""
+    p = Problem(shape, lens, bf16_state, seed=101, pad=pad, shift=shift)
+    pool = p.pool.to(DEV)
+    assert p.call("prefill", pool, None) == 0
+    hs.sync()
+    check_outputs(p, "prefill", f"windows {lens}")
+    assert torch.equal(hs_bits(pool), hs_bits(p.pool.to(DEV)))
+
+
+@pytest.mark.parametrize("bf16_state", [False, True])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_a_draft_that_is_not_finite_leaves_the_rows_before_it(bf16_state, value):
+    """An infinity or a NaN in v of a window's later row: the rows before it, which may be accepted, are right."""
+    clean, bad = (Problem((4, 2, 128, 128), [16, 9, 30], bf16_state, seed=103) for _ in range(2))
+    row, head, lane = 11, 2, 77
+    at = (bad.ahead + row) * bad.stride + 2 * 2 * 128 + head * 128 + lane
+    bad.rows[at] = value
+    for p in (clean, bad):
+        assert p.call("prefill", p.pool.to(DEV), None) == 0
+    hs.sync()
+    got = bad.out_rows()
+    reached = got[row:16, head, lane]
+    assert not bool(torch.isfinite(reached).any())
+    for b, n in enumerate(clean.lens):
+        first = sum(clean.lens[:b])
+        o, _, ao, _ = clean.oracle(b)
+        here = got[first:first + n].clone()
+        if b == 0:
+            here[row:, head, lane] = o[row:, head, lane]
+        within(here, o, 2.0 ** -8 * o.abs() + ((n + 144) * 2.0 ** -24 + 2.0 ** -16) * ao + 1e-30, f"request {b}")
