@@ -170,9 +170,10 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 //     S  <- e^{g n} S + sum_i (e^{g (n-1-i)} v_i) k_i^T
 //
 // and every sum is a product on the matrix cores (16 x 16 x 32, bf16 operands, f32 sums). q, k and v are bf16 already;
-// what is not becomes two or three bf16 terms, so that the products keep the accuracy of f32: the decayed values three (all
-// their 24 bits, in three truncations), the scores and the state two each for the read-out, whose outputs are bf16 (2^-17
-// of their terms). No power of e^g above 1 is formed, so no decay is too fast.
+// what is not (the decayed values, the scores, the state) becomes three bf16 terms, all its 24 bits in three truncations, so
+// that the products keep the accuracy of f32. Two terms for the scores and the state would be 8 % faster (8192 rows of 64 heads
+// 197 us against 214) and 2^-17 of the terms off, more than the rounding of an output whose terms cancel. No power of e^g above 1
+// is formed, so no decay is too fast.
 //
 // A workgroup is one head of one request over one segment of its rows; wave w holds the state's value rows 32 w .. 32 w + 31
 // in accumulators, 32 keys x 32 values of it per lane and four tiles. The rows of q, k and v go from memory straight to LDS,
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // all segments are computed from there at once. k and v are then read twice, the second time from the caches as far as
 // they hold them.
 //
-// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 200 us (under the profiler, cold
+// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 214 us (under the profiler, cold
 // caches: what the segments add 63, the starts 12, the outputs 140). With k and v twice and eight segments' states
 // written and read twice that moves 940 MB, 184 us at the card's copy rate; a tenth fewer vector instructions (remainders
 // by dot products) changed nothing. The windows of 48 requests of up to sixteen rows (bf16 states, only read) 22.7 us, 4.4
@@ -224,6 +225,9 @@ struct PrefillArgs {
 // e^{g n}; 1 for n = 0 also where nothing is remembered (g = -inf).
 __device__ __forceinline__ float fade_of(float g, int n) { return n == 0 ? 1.0f : expf(g * (float)n); }
 
+// A value that is the same in all lanes, held once for the wave.
+__device__ __forceinline__ float uniform(float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); }
+
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 
 __device__ __forceinline__ bf16x8 operand(const uint32_t (&w)[4]) {
@@ -246,16 +250,26 @@ __device__ __forceinline__ f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// N f32 values as hi + lo: hi their upper halves, lo the rest rounded to bf16; two values to a word.
+// N f32 values as three bf16 terms whose sum they are: the upper half of each (8 of its 24 bits), of what remains, and the
+// last 8 bits; two values to a word.
+constexpr int TERMS = 3;
 template <int N>
-__device__ __forceinline__ void two_terms(const float (&x)[N], uint32_t (&hi)[N / 2], uint32_t (&lo)[N / 2]) {
+__device__ __forceinline__ void in_terms(const float (&x)[N], uint32_t (&w)[TERMS][N / 2]) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-        const uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
-        hi[i] = high_halves(a, b);
-        lo[i] = kda::f2bf2(x[2 * i] - __uint_as_float(a & 0xffff0000u), x[2 * i + 1] - __uint_as_float(b & 0xffff0000u));
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int m = 0; m < TERMS; ++m) {
+            const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+            w[m][i] = high_halves(ua, ub);
+            if (m + 1 < TERMS) a -= __uint_as_float(ua & 0xffff0000u), b -= __uint_as_float(ub & 0xffff0000u);
+        }
     }
 }
+
+// The scores' tiles on and below the diagonal, (0, 0), (1, 0) and (1, 1), of one term: where piece `piece` (eight columns) of a
+// row stands. Rows of tile 0 have two pieces, of tile 1 four; sixteen rows at one piece meet every bank once.
+constexpr int SCORES = 3 * 256;
 
 // Where the 16-byte pieces of an LDS row stand: at piece ^ turn(row). Chosen for the two ways of reading: sixteen rows at one
 // piece (a group of lanes that LDS serves at a time then meets every bank once), and four consecutive rows at four consecutive
@@ -266,6 +280,10 @@ __device__ __forceinline__ int turn(int row) {
     if constexpr (PIECES == 16) return (row & 3) << 2 | low;
     if constexpr (PIECES == 8) return (row >> 1 & 1) << 2 | low;
     return low;
+}
+
+__device__ __forceinline__ int score_at(int row, int piece) {
+    return row < 16 ? row * 16 + 8 * (piece ^ (row >> 3)) : 256 + (row - 16) * 32 + 8 * (piece ^ turn<4>(row));
 }
 
 // 16 bytes per lane from global memory to LDS without a register in between: to lds + 16 lane (lds the same in all lanes). Written
@@ -362,7 +380,8 @@ __device__ void outputs_by_rows(const PrefillArgs<S>& a, const S* state, const f
 //
 // Waves per SIMD: three where the rows go straight to LDS, for the sums two and no more, though the registers would let
 // five in: a CU then takes another segment when one of its own ends, which evens out unequal lengths (nine ragged prompts 95 us,
-// with three 97, with five 105).
+// with three 97, with five 105). The outputs' three take 166 of the 168 registers that this leaves them, without a spill: the
+// places in LDS are formed anew from three of them in every chunk.
 //
 // ONCE: windows of one chunk whose states are only read. Nothing is double then, no state is kept behind the product that reads
 // it, and a bf16 state is its operand as it lies in memory, so that more workgroups share a CU's loads (48 windows of up to
@@ -373,16 +392,15 @@ template <typename S, int DK, int NW, bool FAST, bool SUMS, bool ONCE>
 __global__ void __launch_bounds__(64 * NW)
 __attribute__((amdgpu_waves_per_eu(least_waves(FAST, NW, SUMS, ONCE), most_waves(FAST, NW, SUMS, ONCE))))
 segment_kernel(const PrefillArgs<S> a) {
-    constexpr int T = 64 * NW, KT = DK / 16, DV = 32 * NW, TERMS = 3;
+    constexpr int T = 64 * NW, KT = DK / 16, DV = 32 * NW;
     constexpr int KP = DK / 8, VP = DV / 8;                          // pieces of a row
     constexpr int QN = SUMS ? 0 : C * KP / T, KN = C * KP / T, VN = C * VP / T, N = QN + KN + VN;   // pieces per thread and chunk
     static_assert(C * KP % T == 0 && C * VP % T == 0, "whole pieces");
     constexpr int SET = (SUMS ? 1 : 2) * C * DK + C * DV;            // a chunk's rows in LDS: k, v, q
     constexpr int SETS = ONCE ? 1 : 2;
     constexpr bool RAW = ONCE && sizeof(S) == 2;                     // the state's operands as they lie in memory
-    __shared__ __align__(16) bf16_t lds[SETS * SET + (SUMS ? 0 : 2 * C * C)];
-    bf16_t* ph = lds + SETS * SET;                                    // the scores' terms [row][column]
-    bf16_t* pl = ph + C * C;
+    __shared__ __align__(16) bf16_t lds[SETS * SET + (SUMS ? 0 : TERMS * SCORES)];
+    bf16_t* scores = lds + SETS * SET;
     const int h = blockIdx.x % a.heads, seg = blockIdx.x / a.heads, b = blockIdx.y;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), col = lane & 15, grp = lane >> 4;
     const int first = a.cu_rows[b], rows = max(min(a.cu_rows[b + 1] - first, a.most), 0);
@@ -462,9 +480,10 @@ segment_kernel(const PrefillArgs<S> a) {
     // The decays of a whole chunk that this lane uses: of its rows of v to the chunk's end, of the chunk's start to its two
     // rows of outputs, and between the rows of its scores. The score tiles (rows, columns) on and below the diagonal are
     // (0, 0), (1, 0), (1, 1), tile m for wave m mod NW: a wave has tiles of one kind.
-    float in_tail[8], to_row[2], between[4];
+    const float in_tail = fade_of(g, C - 8 - 8 * grp);   // of the last of its eight rows; the others' by steps, alike in all lanes
+    float step[8], to_row[2], between[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) in_tail[e] = fade_of(g, C - 1 - (8 * grp + e));
+    for (int e = 0; e < 8; ++e) step[e] = uniform(fade_of(g, 7 - e));
     if constexpr (!SUMS) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) to_row[i] = a.scale * fade_of(g, 16 * i + col + 1);
@@ -473,23 +492,25 @@ segment_kernel(const PrefillArgs<S> a) {
             const int gap = (wave == 1 ? 16 : 0) + col - (4 * grp + e);
             between[e] = gap < 0 ? 0.0f : a.scale * fade_of(g, gap);
         }
-        for (int i = t; i < C * C / 2; i += T)                       // the tile above the diagonal
-            reinterpret_cast<uint32_t*>(ph)[i] = reinterpret_cast<uint32_t*>(pl)[i] = 0u;
     }
     const float whole = fade_of(g, C);
 
-    // a lane's places in a set: rows col and 16 + col at piece grp (+ 4 u: 32 elements further, under the turn), and transposed rows
-    // 8 grp + col / 4 and four below at piece col mod 4
-    const int at_row = col * DK + 8 * (grp ^ turn<KP>(col)), at_row16 = (16 + col) * DK + 8 * (grp ^ turn<KP>(16 + col));
-    const int tr0 = 8 * grp + (col >> 2), tr1 = tr0 + 4, j = col & 3;
-    const int at_k0 = tr0 * DK + 8 * (j ^ turn<KP>(tr0)), at_k1 = tr1 * DK + 8 * (j ^ turn<KP>(tr1));
-    const int at_v0 = C * DK + tr0 * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr0)), at_v1 = C * DK + tr1 * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr1));
+    // a lane's places in a set: row col at piece grp (+ 4 u: 32 elements further, under the turn; row 16 + col has the same turn),
+    // and transposed row 8 grp + col / 4 at piece col mod 4 (four rows below two pieces further, under the turn)
+    int at_row = col * DK + 8 * (grp ^ turn<KP>(col));
+    const int tr = 8 * grp + (col >> 2), j = col & 3;
+    int at_k = tr * DK + 8 * (j ^ turn<KP>(tr)), at_v = C * DK + tr * DV + 8 * ((4 * wave + j) ^ turn<VP>(tr));
+
+    // its pieces of the scores; the tile above the diagonal is zeros, as the second piece of row 0 always is
+    const int at_p0 = grp < 2 ? score_at(col, grp) : score_at(0, 1), at_p1 = score_at(16 + col, grp);
 
     int set = 0;
     bool odd = false;                             // a chunk's first row shows any infinity or NaN of its v
     for (int c = 0; c * C < n; ++c, set = SET - set) {               // SUMS: chunk n / C - 1 - c
         const int live = SUMS ? C : min(n - c * C, C);
         bf16_t* now = lds + set;
+        // (not known from the chunk before: the compiler would keep every place of a piece in a register of its own)
+        asm volatile("" : "+v"(at_row), "+v"(at_k), "+v"(at_v));
         const bf16_t* qs = now + C * (DK + DV);
         // this thread's part of the chunk is there; behind the barrier everybody's is, and the other set is free
         if constexpr (FAST) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -499,19 +520,22 @@ segment_kernel(const PrefillArgs<S> a) {
 
         // v as an operand: two words of four rows, twice, for each half of the wave's values
         uint32_t vp[2][4];
+        auto load_v = [&] {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            column(now + at_v0 + 4 * x, &vp[x][0]);
-            column(now + at_v1 + 4 * x, &vp[x][2]);
-        }
-        if (live < C) {                           // rows past the last count as zeros
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const int r = 8 * grp + 2 * m;
-                const uint32_t keep = (r < live ? 0x0000ffffu : 0u) | (r + 1 < live ? 0xffff0000u : 0u);
-                vp[0][m] &= keep, vp[1][m] &= keep;
+            for (int x = 0; x < 2; ++x) {
+                column(now + at_v + 4 * x, &vp[x][0]);
+                column(now + (at_v ^ 16) + 4 * DV + 4 * x, &vp[x][2]);
             }
-        }
+            if (live < C) {                       // rows past the last count as zeros
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int r = 8 * grp + 2 * m;
+                    const uint32_t keep = (r < live ? 0x0000ffffu : 0u) | (r + 1 < live ? 0xffff0000u : 0u);
+                    vp[0][m] &= keep, vp[1][m] &= keep;
+                }
+            }
+        };
+        if constexpr (SUMS) load_v();
         if constexpr (!SUMS) {
             // scores: key rows as the first operand, so that a lane holds four consecutive columns of a row
 #pragma unroll
@@ -522,21 +546,21 @@ segment_kernel(const PrefillArgs<S> a) {
                 f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int u = 0; u < DK / 32; ++u)
-                    p = product(operand(now + ((tj ? at_row16 : at_row) ^ (32 * u))), operand(qs + ((ti ? at_row16 : at_row) ^ (32 * u))), p);
+                    p = product(operand(now + (at_row ^ (32 * u)) + 16 * DK * tj), operand(qs + (at_row ^ (32 * u)) + 16 * DK * ti), p);
                 float y[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y[e] = between[e] == 0.0f ? 0.0f : p[e] * between[e];
-                uint32_t hi[2], lo[2];
-                two_terms(y, hi, lo);
-                const int i = 16 * ti + col, jj = 16 * tj + 4 * grp, at = i * C + 8 * ((jj >> 3) ^ turn<4>(i)) + (jj & 7);
-                *reinterpret_cast<uint2*>(ph + at) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(pl + at) = make_uint2(lo[0], lo[1]);
+                uint32_t w[TERMS][2];
+                in_terms(y, w);
+                bf16_t* to = scores + score_at(16 * ti + col, 2 * tj + grp / 2) + 4 * (grp & 1);
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) *reinterpret_cast<uint2*>(to + i * SCORES) = make_uint2(w[i][0], w[i][1]);
             }
             // what the chunk's start gives to its rows
             f32x4 o[2][2] = {};
 #pragma unroll
             for (int u = 0; u < DK / 32; ++u) {
-                const bf16x8 q0 = operand(qs + (at_row ^ (32 * u))), q1 = operand(qs + (at_row16 ^ (32 * u)));
+                const bf16x8 q0 = operand(qs + (at_row ^ (32 * u))), q1 = operand(qs + (at_row ^ (32 * u)) + 16 * DK);
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     if constexpr (RAW) {
@@ -547,25 +571,28 @@ segment_kernel(const PrefillArgs<S> a) {
                     float z[8];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) z[e] = s[2 * u][x][e], z[4 + e] = s[2 * u + 1][x][e];
-                    uint32_t hi[4], lo[4];
-                    two_terms(z, hi, lo);
-                    o[x][0] = product(operand(hi), q0, o[x][0]);
-                    o[x][1] = product(operand(hi), q1, o[x][1]);
-                    o[x][0] = product(operand(lo), q0, o[x][0]);
-                    o[x][1] = product(operand(lo), q1, o[x][1]);
+                    uint32_t w[TERMS][4];
+                    in_terms(z, w);
+#pragma unroll
+                    for (int i = 0; i < TERMS; ++i) {
+                        o[x][0] = product(operand(w[i]), q0, o[x][0]);
+                        o[x][1] = product(operand(w[i]), q1, o[x][1]);
+                    }
                 }
             }
+            load_v();
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int at = (16 * i + col) * C + 8 * (grp ^ turn<4>(16 * i + col));
-                const bf16x8 hi = operand(ph + at), lo = operand(pl + at);
+                bf16x8 p[TERMS];
+#pragma unroll
+                for (int m = 0; m < TERMS; ++m) p[m] = operand(scores + m * SCORES + (i ? at_p1 : at_p0));
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[x][i][e] *= to_row[i];
-                    o[x][i] = product(operand(vp[x]), hi, o[x][i]);
-                    o[x][i] = product(operand(vp[x]), lo, o[x][i]);
+#pragma unroll
+                    for (int m = 0; m < TERMS; ++m) o[x][i] = product(operand(vp[x]), p[m], o[x][i]);
                 }
                 if (16 * i + col < live) {
                     const float y[8] = {o[0][i][0], o[0][i][1], o[0][i][2], o[0][i][3], o[1][i][0], o[1][i][1], o[1][i][2], o[1][i][3]};
@@ -578,27 +605,23 @@ segment_kernel(const PrefillArgs<S> a) {
             if (ONCE || (a.state_out == nullptr && last && (c + 1) * C >= n)) break;   // nobody reads the state behind the last rows
         }
         // v decayed to the chunk's end (SUMS: to the segment's, so that the sums need no decay), in terms
-        uint32_t vd[TERMS][2][4];
+        uint32_t vd[2][TERMS][4];
         {
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = SUMS ? in_tail[e] * fade_of(g, c * C) : in_tail[e];
+            for (int e = 0; e < 8; ++e) f[e] = (SUMS ? in_tail * fade_of(g, c * C) : in_tail) * step[e];
             if (live < C) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) f[e] = fade_of(g, max(live - 1 - (8 * grp + e), 0));
             }
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+            for (int x = 0; x < 2; ++x) {
+                float z[8];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    float z0 = f[2 * m] * __uint_as_float(vp[x][m] << 16), z1 = f[2 * m + 1] * __uint_as_float(vp[x][m] & 0xffff0000u);
-#pragma unroll
-                    for (int i = 0; i < TERMS; ++i) {
-                        const uint32_t r0 = __float_as_uint(z0), r1 = __float_as_uint(z1);
-                        vd[i][x][m] = high_halves(r0, r1);
-                        if (i + 1 < TERMS) z0 -= __uint_as_float(r0 & 0xffff0000u), z1 -= __uint_as_float(r1 & 0xffff0000u);
-                    }
-                }
+                for (int m = 0; m < 4; ++m)
+                    z[2 * m] = f[2 * m] * __uint_as_float(vp[x][m] << 16), z[2 * m + 1] = f[2 * m + 1] * __uint_as_float(vp[x][m] & 0xffff0000u);
+                in_terms(z, vd[x]);
+            }
         }
         // the state behind the chunk
         float by = whole;
@@ -606,14 +629,14 @@ segment_kernel(const PrefillArgs<S> a) {
 #pragma unroll
         for (int m = 0; m < KT; ++m) {
             uint32_t kf[4];
-            column(now + (at_k0 ^ (32 * (m / 2))) + 4 * (m & 1), &kf[0]);
-            column(now + (at_k1 ^ (32 * (m / 2))) + 4 * (m & 1), &kf[2]);
+            column(now + (at_k ^ (32 * (m / 2))) + 4 * (m & 1), &kf[0]);
+            column(now + (at_k ^ (32 * (m / 2) + 16)) + 4 * DK + 4 * (m & 1), &kf[2]);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[m][x][e] *= SUMS ? 1.0f : by;
 #pragma unroll
-                for (int i = 0; i < TERMS; ++i) s[m][x] = product(operand(kf), operand(vd[i][x]), s[m][x]);
+                for (int i = 0; i < TERMS; ++i) s[m][x] = product(operand(kf), operand(vd[x][i]), s[m][x]);
             }
         }
     }
