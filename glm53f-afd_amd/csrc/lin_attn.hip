@@ -481,6 +481,7 @@ segment_kernel(const PrefillArgs<S> a) {
     // rows of outputs, and between the rows of its scores. The score tiles (rows, columns) on and below the diagonal are
     // (0, 0), (1, 0), (1, 1), tile m for wave m mod NW: a wave has tiles of one kind.
     const float in_tail = fade_of(g, C - 8 - 8 * grp);   // of the last of its eight rows; the others' by steps, alike in all lanes
+    const int gap = (wave == 1 ? 16 : 0) + col - 4 * grp;   // from the first of its scores' four rows of k to their row of q
     float step[8], to_row[2], between[4];
 #pragma unroll
     for (int e = 0; e < 8; ++e) step[e] = uniform(fade_of(g, 7 - e));
@@ -488,10 +489,7 @@ segment_kernel(const PrefillArgs<S> a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) to_row[i] = a.scale * fade_of(g, 16 * i + col + 1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int gap = (wave == 1 ? 16 : 0) + col - (4 * grp + e);
-            between[e] = gap < 0 ? 0.0f : a.scale * fade_of(g, gap);
-        }
+        for (int e = 0; e < 4; ++e) between[e] = a.scale * fade_of(g, max(gap - e, 0));
     }
     const float whole = fade_of(g, C);
 
@@ -549,7 +547,7 @@ segment_kernel(const PrefillArgs<S> a) {
                     p = product(operand(now + (at_row ^ (32 * u)) + 16 * DK * tj), operand(qs + (at_row ^ (32 * u)) + 16 * DK * ti), p);
                 float y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = between[e] == 0.0f ? 0.0f : p[e] * between[e];
+                for (int e = 0; e < 4; ++e) y[e] = gap < e ? 0.0f : p[e] * between[e];   // (a decay of 0 keeps a NaN)
                 uint32_t w[TERMS][2];
                 in_terms(y, w);
                 bf16_t* to = scores + score_at(16 * ti + col, 2 * tj + grp / 2) + 4 * (grp & 1);
