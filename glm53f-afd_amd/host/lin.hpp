@@ -87,7 +87,8 @@ struct Attention {
         auto off = [](const Request& r) { return r.state_offset; };
         for (const Request& r : meta.requests())
             if (r.state_offset % 8) return Error::invalid("state offsets are multiples of 8 elements");
-        KDA_TRY(meta.check_regions("state", state, es, 0, shape.state_len(), true, off));
+        // (windows that only read their states may stand behind the same one)
+        KDA_TRY(meta.check_regions("state", state, es, 0, shape.state_len(), state_out.kind != StateOut::Skip, off));
         *state_out_ptr = nullptr;
         if (state_out.kind == StateOut::InPlace) {
             *state_out_ptr = state.p;
