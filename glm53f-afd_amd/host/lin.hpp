@@ -1,6 +1,7 @@
 // Checked wrappers over linear attention with one decay per head (include/ext/glm53f_lin.h), in the manner of kernel.hpp:
-// every launch first checks on the host that each buffer holds the geometry it is given and that written regions do not
-// overlap, then makes one call into the C ABI. check() never touches the GPU. The batch metadata is kernel.hpp's BatchMeta
+// every launch first checks on the host that each buffer holds the geometry it is given and that the states written overlap
+// neither each other nor one that another request reads, then makes one call into the C ABI. (That `out` lies apart from q, k
+// and v is the caller's, as there.) check() never touches the GPU. The batch metadata is kernel.hpp's BatchMeta
 // (its conv offsets are not used), so that one set of requests serves layers of both kinds. Header only.
 #ifndef GLM53F_LIN_HOST_LIN_HPP
 #define GLM53F_LIN_HOST_LIN_HPP
@@ -96,6 +97,7 @@ struct Attention {
             if (state_out.offset != 0) return Error::invalid("a batch writes its states at the requests' offsets");
             KDA_TRY(meta.check_regions("state_out", state_out.buf, es, 0, shape.state_len(), true, off));
             if (glm53f_kda::same(state_out.buf, state)) return Error::invalid("state_out is the state buffer: use InPlace");
+            KDA_TRY(check_apart(meta, es));
             *state_out_ptr = state_out.buf.p;
         }
         return Error::ok();
@@ -141,6 +143,20 @@ struct Attention {
     }
 
   private:
+    /// The states that go to state_out lie apart from every state that is read, whatever the two buffers share.
+    Error check_apart(const BatchMeta& meta, size_t es) const {
+        const uintptr_t bytes = shape.state_len() * es;
+        std::vector<uintptr_t> read;
+        for (const Request& r : meta.requests()) read.push_back((uintptr_t)state.p + r.state_offset * es);
+        std::sort(read.begin(), read.end());
+        for (const Request& r : meta.requests()) {
+            const uintptr_t at = (uintptr_t)state_out.buf.p + r.state_offset * es;
+            const auto next = std::upper_bound(read.begin(), read.end(), at);
+            if ((next != read.begin() && at - next[-1] < bytes) || (next != read.end() && *next - at < bytes))
+                return Error::invalid("state_out overlaps a state that is read");
+        }
+        return Error::ok();
+    }
     int32_t h() const { return (int32_t)shape.heads; }
     int32_t qk() const { return (int32_t)shape.qk_heads; }
     int32_t dk() const { return (int32_t)shape.key_dim; }

@@ -56,8 +56,31 @@ static void windows_of_one_state() {
     EXPECT(kind(a, meta) == Error::Invalid);            // outside the pool
 }
 
+// States written to another buffer lie apart from every state that is read, also where the buffers are parts of one allocation.
+static void states_written_elsewhere() {
+    const size_t n = kShape.state_len(), bytes = n * 4;
+    BatchMeta meta(3);
+    EXPECT(meta.set({{2, 0, n}, {1, 0, 3 * n}, {0, 0, 5 * n}}).is_ok());
+    Attention a = attention(3);
+    auto to = [&](uintptr_t at, size_t size) { a.state_out = StateOut::to(fake(size, at)); return kind(a, meta); };
+    EXPECT(to(2 * kPool, 6 * bytes) == Error::Ok);
+    EXPECT(to(kPool + 6 * bytes, 6 * bytes) == Error::Ok && to(kPool - 6 * bytes, 6 * bytes) == Error::Ok);
+    EXPECT(to(kPool + bytes, 6 * bytes) == Error::Ok && to(kPool - bytes, 6 * bytes) == Error::Ok);   // the slots between
+    EXPECT(to(kPool + 2 * bytes, 6 * bytes) == Error::Invalid);      // the next request's
+    EXPECT(to(kPool - 4 * bytes, 6 * bytes) == Error::Invalid);
+    EXPECT(to(kPool + 16, 6 * bytes) == Error::Invalid && to(kPool - 16, 6 * bytes) == Error::Invalid);   // its own in part
+    EXPECT(to(kPool + bytes + 16, 6 * bytes) == Error::Invalid && to(kPool + bytes - 16, 6 * bytes) == Error::Invalid);
+    EXPECT(to(kPool, 6 * bytes) == Error::Invalid);                  // InPlace
+    a.state = fake(6 * n * 2, kPool);
+    a.state_out = StateOut::to(fake(6 * n * 2, kPool + n * 2));
+    EXPECT(kind(a, meta, StateType::Bf16) == Error::Ok);
+    a.state_out = StateOut::to(fake(6 * n * 2, kPool + 2 * n * 2));
+    EXPECT(kind(a, meta, StateType::Bf16) == Error::Invalid);
+}
+
 int main() {
     windows_of_one_state();
+    states_written_elsewhere();
     if (failures) { std::printf("%d failures\n", failures); return 1; }
     std::printf("state checks passed\n");
     return 0;
