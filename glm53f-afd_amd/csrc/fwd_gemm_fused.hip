@@ -337,8 +337,9 @@ int32_t stream_tiles(const Args& a) {
     return stream<CK, NT, 1, KS, ANY>(a);
 }
 
-// The waves per workgroup, which split k: eight where one tile each is at most a workgroup per CU, four otherwise, one
-// where k is short; chunks of 256 where every wave has whole ones.
+// The waves per workgroup, which split k: eight where one tile each is at most a workgroup per CU and k is 1024 at least, four
+// otherwise, one below 512; chunks of 256 where every wave has whole ones. The aligned form's waves have equal shares of whole
+// chunks (whole_shares); the form for any address cuts the chunks as evenly as they go.
 template <int NT, int TMAX, bool ANY>
 int32_t stream_split(const Args& a) {
     const long long tiles = (long long)((a.n + 15) / 16) * a.groups;
@@ -353,6 +354,16 @@ int32_t stream_split(const Args& a) {
         return stream_tiles<128, NT, 4, TMAX, ANY>(a);
     }
     return stream_tiles<128, NT, 1, TMAX, ANY>(a);
+}
+
+// The aligned form would need fewer waves for other k, and loses more by that than it gains by its loads (us, aligned and any):
+//   1, 16, 64 rows 11,008 -> 4096 with one wave   52 52 99    any  19 21 34
+//   1, 16, 64 rows 640 -> 4096 with one wave      5.2 5.3 9.4      5.0 4.9 5.2
+//   1, 16, 64 rows 5632 -> 2048 with four waves   9.9 10.0 18.3    6.7 7.1 12.8
+//   1, 16, 64 rows 5632 -> 4096 with four waves   10.9 11.0 19.2   10.4 11.7 18.6
+bool whole_shares(const Args& a) {
+    const long long tiles = (long long)((a.n + 15) / 16) * a.groups;
+    return a.k < 512 || a.k % (tiles <= kCus && a.k >= 1024 ? 1024 : 512) == 0;
 }
 
 template <bool ANY>
@@ -456,10 +467,11 @@ extern "C" int32_t glm53f_fwd_gemm_bf16_fused(const uint16_t* x, int64_t ldx, in
     const bool fast = aligned(x, 16) && aligned(w, 16) && ldx % 8 == 0 && ldw % 8 == 0 && x_gstride % 8 == 0 &&
                       w_gstride % 8 == 0;
     // Up to 64 rows the weights stream past the rows once; with up to 256 too where a workgroup per sixteen outputs and 64 rows is at
-    // most one per CU (200 rows 4096 -> 512: 10.9 us against 13.1 with tiles; 128 rows 8192 -> 2048 20.6 and 25.3; 128 rows
-    // 512 -> 1024 4.8 and 4.9).
+    // most one per CU and k is long enough for more than one wave (200 rows 4096 -> 512: 10.9 us against 13.1 with tiles; 128 rows
+    // 8192 -> 2048 20.6 and 25.3, 11,008 -> 1024 20.9 and 27.9, 1001 -> 1024 6.1 and 7.8, 640 -> 2048 4.7 and 4.9; but 384 -> 1024 6.3
+    // and 4.5, 136 -> 512 6.5 and 4.6).
     const long long thin = (long long)((n + 15LL) / 16) * ((rows + 63LL) / 64) * groups;
-    if (rows <= 64 || (rows <= 256 && thin <= kCus))
-        return fast && n % 16 == 0 && k % 128 == 0 ? stream_rows<false>(a) : stream_rows<true>(a);
+    if (rows <= 64 || (rows <= 256 && thin <= kCus && k >= 512))
+        return fast && n % 16 == 0 && k % 128 == 0 && whole_shares(a) ? stream_rows<false>(a) : stream_rows<true>(a);
     return tiled(a, fast && k % 8 == 0);
 }
