@@ -326,15 +326,15 @@ int32_t stream(const Args& a) {
     return (int32_t)hipGetLastError();
 }
 
-// The weight tiles per workgroup: the power of two (at most TMAX) that brings the grid nearest to one workgroup per CU
+// The weight tiles per workgroup: the power of two (TMIN to TMAX) that brings the grid nearest to one workgroup per CU
 // from above.
-template <int CK, int NT, int KS, int TMAX, bool ANY>
+template <int CK, int NT, int KS, int TMIN, int TMAX, bool ANY>
 int32_t stream_tiles(const Args& a) {
     const long long tiles = (long long)((a.n + 15) / 16) * a.groups;
     if constexpr (TMAX >= 8) if (tiles > 4 * kCus) return stream<CK, NT, 8, KS, ANY>(a);
     if constexpr (TMAX >= 4) if (tiles > 2 * kCus) return stream<CK, NT, 4, KS, ANY>(a);
-    if constexpr (TMAX >= 2) if (tiles > kCus) return stream<CK, NT, 2, KS, ANY>(a);
-    return stream<CK, NT, 1, KS, ANY>(a);
+    if constexpr (TMIN < 2) if (tiles > kCus) return stream<CK, NT, 2, KS, ANY>(a);
+    return stream<CK, NT, TMIN, KS, ANY>(a);
 }
 
 // The waves per workgroup, which split k: eight where one tile each is at most a workgroup per CU and k is 1024 at least, four
@@ -346,14 +346,14 @@ int32_t stream_split(const Args& a) {
     if (tiles <= kCus && (ANY ? a.k >= 1024 : a.k % 1024 == 0)) {
         // (sixteen rows a workgroup where they still are at most one per CU: 192 rows 2048 -> 1024 10.8 us otherwise, 7.7 so)
         const long long row_tiles = a.rows <= 64 ? NT : (a.rows + 15) / 16;
-        if (!ANY && a.k % 2048 == 0 && (NT == 1 || tiles * row_tiles <= kCus)) return stream<256, 1, 1, 8, ANY>(a);
+        if constexpr (!ANY) if (a.k % 2048 == 0 && (NT == 1 || tiles * row_tiles <= kCus)) return stream<256, 1, 1, 8, ANY>(a);
         return stream<128, NT, 1, 8, ANY>(a);
     }
     if (ANY ? a.k >= 512 : a.k % 512 == 0) {
-        if (!ANY && a.k % 1024 == 0) return stream_tiles<256, NT, 4, 8, ANY>(a);
-        return stream_tiles<128, NT, 4, TMAX, ANY>(a);
+        if constexpr (!ANY) if (a.k % 1024 == 0) return stream_tiles<256, NT, 4, 2, 8, ANY>(a);   // (more tiles than CUs)
+        return stream_tiles<128, NT, 4, 1, TMAX, ANY>(a);
     }
-    return stream_tiles<128, NT, 1, TMAX, ANY>(a);
+    return stream_tiles<128, NT, 1, 1, TMAX, ANY>(a);
 }
 
 // The aligned form would need fewer waves for other k, and loses more by that than it gains by its loads (us, aligned and any):
