@@ -71,8 +71,11 @@ def reached():
 
 
 def cheapest():
-    """Every kernel with the sizes of the least work that reach it: {kernel: (rows, n, k, aligned)}."""
+    """Every kernel with the sizes of the least work that reach it, {kernel: (rows, n, k, aligned)}: tiles with several steps
+    of k, of rows at any address an odd k."""
     found = {}
     for r, n, k, a in sorted(sizes(), key=lambda s: (s[0] + 64) * s[1] * s[2]):
-        found.setdefault(kernel_of(r, n, k, 1, a), (r, n, k, a))
+        kernel = kernel_of(r, n, k, 1, a)
+        if kernel[0] == "stream" or (k > 512 if a else k % 2):
+            found.setdefault(kernel, (r, n, k, a))
     return found
