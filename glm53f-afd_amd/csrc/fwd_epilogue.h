@@ -29,16 +29,21 @@ __device__ __forceinline__ float gated(float y, float z) {
     return y * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
 }
 
-// y Phi(y), with erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2), t = 1 / (1 + 0.3275911 x) for x >= 0 (Abramowitz and Stegun,
-// Handbook of Mathematical Functions, 7.1.26: off by at most 1.5e-7); the far left keeps the factor e^(-x^2). A sixth of the
-// instructions of the library's erfc: 333 rows 1001 -> 1999 take 4 us less.
+// y Phi(y), with e^(x^2) erfc(x) / 2 = t (c0 + c1 t + .. + c8 t^8), t = 1 / (1 + 0.4 x) for x >= 0: the polynomial of least
+// relative error over all x (weighted least squares, the weights raised where the error is largest), off by at most 1.3e-7 of the
+// value, so that the far left, which keeps the factor e^(-x^2), stays accurate too. 333 rows 1001 -> 1999 take 12.1 us with it, as
+// with five terms that are 5e-5 of the value off at y = -3; the library's erfc took 4 us more.
 __device__ __forceinline__ float gelu(float y) {
-    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(y), 1.0f));
-    float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-    p = __builtin_fmaf(p, t, 1.421413741f);
-    p = __builtin_fmaf(p, t, -0.284496736f);
-    p = __builtin_fmaf(p, t, 0.254829592f);
-    const float half = 0.5f * p * t * __builtin_amdgcn_exp2f(y * y * -0.72134752044448170f);   // erfc(|y| / sqrt 2) / 2
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.4f * 0.70710678118654752f, fabsf(y), 1.0f));
+    float p = __builtin_fmaf(0.0251339953f, t, -0.0914624855f);
+    p = __builtin_fmaf(p, t, 0.0845619738f);
+    p = __builtin_fmaf(p, t, -0.00282036117f);
+    p = __builtin_fmaf(p, t, 0.070723772f);
+    p = __builtin_fmaf(p, t, 0.0842687935f);
+    p = __builtin_fmaf(p, t, 0.103921659f);
+    p = __builtin_fmaf(p, t, 0.112834781f);
+    p = __builtin_fmaf(p, t, 0.112837933f);
+    const float half = p * t * __builtin_amdgcn_exp2f(y * y * -0.72134752044448170f);   // erfc(|y| / sqrt 2) / 2
     return y * (y < 0.0f ? half : 1.0f - half);
 }
 
