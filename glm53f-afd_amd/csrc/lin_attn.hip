@@ -35,8 +35,7 @@ __device__ __forceinline__ void load_row(const bf16_t* p, bf16_t (&e)[N]) {
     }
 }
 
-// PAST: past the caches.
-template <int N, bool PAST = false>
+template <int N>
 __device__ __forceinline__ void store_row(bf16_t* p, const float (&x)[N]) {
     if constexpr (N == 1) {
         p[0] = kda::f2bf(x[0]);
@@ -48,8 +47,7 @@ __device__ __forceinline__ void store_row(bf16_t* p, const float (&x)[N]) {
             vec w;
 #pragma unroll
             for (int c = 0; c < V / 2; ++c) w[c] = kda::f2bf2(x[i + 2 * c], x[i + 2 * c + 1]);
-            if constexpr (PAST) __builtin_nontemporal_store(w, reinterpret_cast<vec*>(p + i));
-            else *reinterpret_cast<vec*>(p + i) = w;
+            *reinterpret_cast<vec*>(p + i) = w;
         }
     }
 }
@@ -219,7 +217,6 @@ struct PrefillArgs {
     ll out_stride;
     float* work;                                  // [batch][heads][segs] states in the waves' order, NULL: one segment
     int segs, seg_rows;                           // seg_rows: a multiple of C
-    int past;                                     // the outputs go past the caches
 };
 
 // e^{g n}; 1 for n = 0 also where nothing is remembered (g = -inf).
@@ -595,8 +592,7 @@ segment_kernel(const PrefillArgs<S> a) {
                 if (16 * i + col < live) {
                     const float y[8] = {o[0][i][0], o[0][i][1], o[0][i][2], o[0][i][3], o[1][i][0], o[1][i][1], o[1][i][2], o[1][i][3]};
                     bf16_t* at = a.out + (row0 + c * C + 16 * i + col) * a.out_stride + (ll)h * DV + 32 * wave + 8 * grp;
-                    if (a.past) store_row<8, true>(at, y);
-                    else store_row<8>(at, y);
+                    store_row<8>(at, y);
                 }
             }
             odd |= !finite(o[0][0], o[1][0]);
@@ -728,7 +724,10 @@ int chain(int heads, int qk_heads, int dk, int dv, int batch, ChainArgs<S> a, hi
 }
 
 // Segments of a call: as many as give every CU two workgroups, or with several requests four, so that requests of unequal
-// length even out; a segment is 256 rows at least, since one costs a state's round through memory. Sizes alone decide.
+// length even out; a segment is 256 rows at least, since one costs a state's round through memory. Sizes alone decide, and they do
+// not say whether the requests are alike. Two and four workgroups, us (64 heads of 128 but for the last two): one prompt of 8192
+// rows 220 and 238; three of up to 4096 rows 281 and 240; nine of up to 1801 (32 heads, 64 keys) 132 and 100; but several equal
+// ones 2 x 8192 400 and 423, 4 x 2048 203 and 231, 20 x 600 of 16 heads 79 and 123.
 struct Cut {
     int segs, seg_rows;
 };
@@ -771,12 +770,9 @@ int prefill(int heads, int qk_heads, int dk, int dv, int batch, int max_rows, co
     if (c.segs > 1 && (!workspace || !aligned(workspace, 16) ||
                        workspace_bytes < glm53f_lin_prefill_workspace_bytes(heads, dk, dv, batch, max_rows)))
         return kInvalid;
-    // Segments read k and v twice. Where they are about as large as the cache behind the L2 the outputs, written meanwhile, go
-    // past it (k and v of 268 MB: 204 us with them in, 198 past; of 100 MB 95 and 100).
-    const bool past = c.segs > 1 && (ll)batch * max_rows * ((ll)heads * dv + (ll)qk_heads * dk) * (ll)sizeof(bf16_t) > 192LL << 20;
     const PrefillArgs<S> a{heads, heads / qk_heads, max_rows, r.cu_rows, r.q, r.q_stride, r.k, r.k_stride, r.v, r.v_stride,
                            r.log_decay, r.scale, r.state_in, r.state_out, r.state_off, r.out, r.out_stride,
-                           c.segs > 1 ? static_cast<float*>(workspace) : nullptr, c.segs, c.seg_rows, past ? 1 : 0};
+                           c.segs > 1 ? static_cast<float*>(workspace) : nullptr, c.segs, c.seg_rows};
     const bool fast = whole_pieces(r.q, r.q_stride) && whole_pieces(r.k, r.k_stride) && whole_pieces(r.v, r.v_stride);
     return dk == 64 ? launch_prefill<S, 64>(a, dv, fast, batch, stream) : launch_prefill<S, 128>(a, dv, fast, batch, stream);
 }

@@ -1,5 +1,4 @@
-"""Linear attention with one decay per head, a prompt whose keys and values are larger than the caches behind the L2 (its
-outputs then go past them): rows and states of some heads against the recurrence in 64 bits, all others finite, and what
+"""Linear attention with one decay per head, a prompt whose keys and values are larger than the caches behind the L2: rows and states of some heads against the recurrence in 64 bits, all others finite, and what
 lies around the rows as it was.
 
 Tolerances as for any prompt: R rows bring at most R roundings of 2^-24 to a state's entry, a read-out key_dim more and the
@@ -20,7 +19,7 @@ DEV = hs.DEV
 
 
 @pytest.mark.parametrize("shift", [0, 1])
-def test_outputs_past_the_caches(shift):
+def test_a_prompt_larger_than_the_caches(shift):
     heads, d, rows = 64, 128, 6301
     assert rows * heads * d * 2 * 2 > 192 << 20
     gen = torch.Generator().manual_seed(rows)
