@@ -1,6 +1,6 @@
 """Every kernel that the fused product can launch, each at the sizes of least work that reach it, with bias, an activation
 and the residual, in place too, both output types, and its last rows and columns whole tiles or not: against 64-bit
-arithmetic. And the tiles' addresses beyond 2^31 elements.
+arithmetic. And addresses beyond 2^31 elements.
 
 Tolerance: (k + 1) roundings of 2^-24 of the absolute sum whatever the order, an activation's slope of at most 1.13 and its
 own evaluation within 2^-20 (1 + |y|), and one rounding each for the residual and the outputs (f32 2^-24, bf16 2^-8)."""
@@ -58,10 +58,11 @@ def test_kernel(kernel, size, f32_out, in_place):
 
 @pytest.mark.parametrize("shift", [0, 1])
 @pytest.mark.parametrize("f32_out", [False, True])
-def test_tiles_beyond_31_bits(shift, f32_out):
-    """Rows of x, of the residual and of the outputs further than 2^31 elements apart, more of them than the streaming kernels take."""
-    rows, n, k, stride = 300, 64, 128, (1 << 23) + 8           # 299 strides: 2.5e9 elements
-    assert fd.kernel_of(rows, n, k, 1, shift == 0)[0] == "tile"
+@pytest.mark.parametrize("kind_of_kernel,rows,stride", [("tile", 300, (1 << 23) + 8), ("stream", 40, (1 << 26) + 8)])
+def test_rows_beyond_31_bits(kind_of_kernel, rows, stride, shift, f32_out):
+    """Rows of x, of the residual and of the outputs further than 2^31 elements apart (2.5e9 and 2.6e9)."""
+    n, k = 64, 128
+    assert fd.kernel_of(rows, n, k, 1, shift == 0)[0] == kind_of_kernel
     gen = torch.Generator().manual_seed(shift)
     kind = torch.float32 if f32_out else torch.bfloat16
     x, w = torch.randn(rows, k, generator=gen).bfloat16(), torch.randn(n, k, generator=gen).bfloat16()
