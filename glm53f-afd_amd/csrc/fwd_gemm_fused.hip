@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(64 * WM * WN * KW) tile_kernel(const Args a) {
             }
     };
     // The residual's tile is asked for during the last steps, into a corner that nobody reads: the epilogue then finds it in the
-    // caches (2048 rows 8192 -> 4096 134 -> 129 us, 124 without a residual; 1024 -> 4096 41 -> 37; 4096 rows 4096 -> 8192
-    // 313 -> 295).
+    // caches (2048 rows 8192 -> 4096 134 -> 132 us, 129 without a residual; 1024 -> 4096 34.6 -> 33.1; 4096 rows 4096 -> 8192
+    // 318 -> 298; 256 rows 4096 -> 4096 22.1 -> 21.2).
     const int res = a.e.early ? (a.e.out_f32 ? BM * BN / 4 / T : BM * BN / 8 / T) : 0, res_from = max(steps - res - 4, 0);
     auto early = [&](int step) {
         const int i = step - res_from, per = a.e.out_f32 ? 4 : 8, slot = i * T + t;

@@ -185,11 +185,11 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // all segments are computed from there at once. k and v are then read twice, the second time from the caches as far as
 // they hold them.
 //
-// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 214 us (under the profiler, cold
-// caches: what the segments add 63, the starts 12, the outputs 140). With k and v twice and eight segments' states
-// written and read twice that moves 940 MB, 184 us at the card's copy rate; a tenth fewer vector instructions (remainders
-// by dot products) changed nothing. The windows of 48 requests of up to sixteen rows (bf16 states, only read) 22.7 us, 4.4
-// TB/s of states.
+// Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 214 to 225 us from one
+// machine to another (under the profiler, which leaves lower clocks and colder caches: what the segments add 64, the starts 14, the
+// outputs 189). With k and v twice and eight segments' states written and read twice that moves 940 MB, 184 us at the card's copy
+// rate; the products and the splitting into terms no longer hide behind it (two terms 8 % faster). The windows of 48 requests of up
+// to sixteen rows (bf16 states, only read) 23 us, 4.4 TB/s of states; with f32 states 102 us with their commit.
 
 constexpr int C = 32;                             // rows per chunk: one product's depth
 
@@ -376,13 +376,13 @@ __device__ void outputs_by_rows(const PrefillArgs<S>& a, const S* state, const f
 // the state. FAST: the rows of q, k and v are 16-byte aligned and go straight to LDS; otherwise through registers.
 //
 // Waves per SIMD: three where the rows go straight to LDS, for the sums two and no more, though the registers would let
-// five in: a CU then takes another segment when one of its own ends, which evens out unequal lengths (nine ragged prompts 95 us,
-// with three 97, with five 105). The outputs' three take 166 of the 168 registers that this leaves them, without a spill: the
-// places in LDS are formed anew from three of them in every chunk.
+// five in: a CU then takes another segment when one of its own ends, which evens out unequal lengths (nine ragged prompts 99 us,
+// with three 102, with five 114; equal ones alike). The outputs' three take 166 of the 168 registers that this leaves them,
+// without a spill: the places in LDS are formed anew from three of them in every chunk.
 //
 // ONCE: windows of one chunk whose states are only read. Nothing is double then, no state is kept behind the product that reads
 // it, and a bf16 state is its operand as it lies in memory, so that more workgroups share a CU's loads (48 windows of up to
-// sixteen rows of 64 heads, bf16 states: 22.7 us against 34).
+// sixteen rows of 64 heads, bf16 states: 23 us against 34).
 constexpr int least_waves(bool fast, int nw, bool sums, bool once) { return once ? (nw == 4 ? 4 : 2) : fast && nw == 4 && !sums ? 3 : 2; }
 constexpr int most_waves(bool fast, int nw, bool sums, bool once) { return fast && nw == 4 && !once ? (sums ? 2 : 3) : 8; }
 template <typename S, int DK, int NW, bool FAST, bool SUMS, bool ONCE>

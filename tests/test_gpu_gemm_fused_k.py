@@ -43,15 +43,17 @@ def product(rows, n, k, pad, seed, groups=1, act=2):
 
 
 @pytest.mark.parametrize("k", [640, 896, 1152, 1536, 2560, 5248, 11008])
-@pytest.mark.parametrize("rows,n", [(1, 1024), (16, 4096), (17, 208), (33, 1040), (64, 4112), (40, 8208)])
-def test_k_of_whole_chunks_but_no_equal_shares(rows, n, k):
-    product(rows, n, k, 8, rows + k)
+def test_k_of_whole_chunks_but_no_equal_shares(k):
+    for rows, n in ((1, 1024), (16, 4096), (17, 208), (33, 1040), (64, 4112), (40, 8208)):
+        print(f"{rows} rows {k} -> {n}", flush=True)
+        product(rows, n, k, 8, rows + k)
 
 
 @pytest.mark.parametrize("k", [8, 136, 384, 504, 512, 520, 640, 1152, 2176])
-@pytest.mark.parametrize("rows,n", [(65, 512), (100, 1024), (200, 2048), (256, 1024), (129, 333)])
-def test_thin_products_of_more_rows(rows, n, k):
-    product(rows, n, k, 8, rows + k)
+def test_thin_products_of_more_rows(k):
+    for rows, n in ((65, 512), (100, 1024), (200, 2048), (256, 1024), (129, 333)):
+        print(f"{rows} rows {k} -> {n}", flush=True)
+        product(rows, n, k, 8, rows + k)
 
 
 @pytest.mark.parametrize("rows", [7, 50, 90])

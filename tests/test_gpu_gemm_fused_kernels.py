@@ -31,10 +31,14 @@ def check(got, x, w, b, r, act, f32_out):
 
 
 @pytest.mark.parametrize("kernel,size", CASES, ids=["-".join(str(int(v) if isinstance(v, bool) else v) for v in k) for k, _ in CASES])
-@pytest.mark.parametrize("f32_out,in_place", [(False, True), (True, False), (True, True)])
-def test_kernel(kernel, size, f32_out, in_place):
-    rows, n, k, aligned = size
-    assert fd.kernel_of(rows, n, k, 1, aligned) == kernel
+def test_kernel(kernel, size):
+    assert fd.kernel_of(*size[:3], 1, size[3]) == kernel
+    for f32_out, in_place in ((False, True), (True, False), (True, True)):
+        print(f"{kernel} {size} f32 {f32_out} in place {in_place}", flush=True)
+        run(*size, f32_out, in_place)
+
+
+def run(rows, n, k, aligned, f32_out, in_place):
     shift = 0 if aligned else 1
     gen = torch.Generator().manual_seed(rows + n + k)
     kind = torch.float32 if f32_out else torch.bfloat16
