@@ -169,9 +169,9 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 //
 // and every sum is a product on the matrix cores (16 x 16 x 32, bf16 operands, f32 sums). q, k and v are bf16 already;
 // what is not (the decayed values, the scores, the state) becomes three bf16 terms, all its 24 bits in three truncations, so
-// that the products keep the accuracy of f32. Two terms for the scores and the state would be 8 % faster (8192 rows of 64 heads
-// 197 us against 214) and 2^-17 of the terms off, more than the rounding of an output whose terms cancel. No power of e^g above 1
-// is formed, so no decay is too fast.
+// that the products keep the accuracy of f32. Two terms for the scores and the state would be 4 to 11 % faster (8192 rows of 64
+// heads 197 us against 214, nine ragged prompts 93 and 97, six of up to 700 rows of 16 heads with 64 values 44 and 49) and 2^-17 of
+// the terms off, more than the rounding of an output whose terms cancel. No power of e^g above 1 is formed, so no decay is too fast.
 //
 // A workgroup is one head of one request over one segment of its rows; wave w holds the state's value rows 32 w .. 32 w + 31
 // in accumulators, 32 keys x 32 values of it per lane and four tiles. The rows of q, k and v go from memory straight to LDS,
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(THREADS) chain_kernel(const ChainArgs<S> a) {
 // Measured on 8192 rows of 64 heads of 128 (k and v 268 MB, with q and the outputs 537 MB): 214 to 225 us from one
 // machine to another (under the profiler, which leaves lower clocks and colder caches: what the segments add 64, the starts 14, the
 // outputs 189). With k and v twice and eight segments' states written and read twice that moves 940 MB, 184 us at the card's copy
-// rate; the products and the splitting into terms no longer hide behind it (two terms 8 % faster). The windows of 48 requests of up
+// rate; the products and the splitting into terms do not all hide behind it. The windows of 48 requests of up
 // to sixteen rows (bf16 states, only read) 23 us, 4.4 TB/s of states; with f32 states 102 us with their commit.
 
 constexpr int C = 32;                             // rows per chunk: one product's depth
